@@ -391,6 +391,21 @@ int fg_attention_prefill_tc_variant(int bits);   /* bit 0 / 1: two score tiles a
 int fg_attention_prefill_tc_test_hook(long long wait_limit_cycles, int skip_copy);   /* tests only */
 /* fg_attention_decode_noalloc: see fastgguf_noalloc.h */
 
+/* ---- libfg_mx: matrices in microscaled 4-bit floating point.  data [rows, K / 2] bytes, scales [ceil(rows / 128), ceil(K / 128), 32, 4, 4]
+   bytes (mxfp4.cuh), both 16-byte aligned; K a multiple of 32; strides count numbers */
+/* mats matrices [R, K] of dtype (rows ldx, matrices x_stride apart) to data and scales, one matrix after another */
+int fg_mxfp4_quantize(const void *x, int dtype, long long ldx, long long x_stride, void *data, void *scales, int mats, int R, int K,
+                      cudaStream_t stream);
+/* out[i] = scale * row rows[i] (rows null: row i), i < n, of a matrix [R, K]; an index outside the matrix gives a row of NaN */
+int fg_mxfp4_rows(const void *data, const void *scales, const int *rows, void *out, int out_dtype, long long ldo, int n, int R, int K,
+                  float scale, cudaStream_t stream);
+/* out (+)= x w^T: x [M, K] bfloat16, w [N, K]; out bfloat16 or float32, accumulate: float32 alone */
+int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
+                  int M, int N, int K, cudaStream_t stream);
+/* rows offsets[e] <= m < offsets[e + 1] (device) with matrix e of a stack; rows of no run are not written */
+int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w, const void *scales, const int *offsets, int experts, void *out,
+                          int out_dtype, long long ldo, int accumulate, int M, int N, int K, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,10 +7,12 @@ from typing import Optional
 import torch
 
 from .lib import KernelError, check, dtype_code, lib, ptr, raise_on_device_error, require_cuda, stream
+from .mxfp4 import Mxfp4, gemm_mxfp4, gemm_mxfp4_both, gemm_mxfp4_grouped, mxfp4_quantize, mxfp4_rows
 
 __all__ = [
     "KernelError", "raise_on_device_error", "embed_gather", "embed_gather_norm", "rmsnorm", "rope_append", "silu_mul", "gemm_generic",
     "attention_generic", "attention", "rope_attention", "sample", "argmax", "decode_advance",
+    "Mxfp4", "mxfp4_quantize", "mxfp4_rows", "gemm_mxfp4", "gemm_mxfp4_both", "gemm_mxfp4_grouped",
 ]
 
 

@@ -1,0 +1,231 @@
+"""Weights in microscaled 4-bit floating point (MXFP4): quantising rows, reading rows back (also the lookup in an embedding table), and the
+contractions of a decoder on such weights.
+
+A number is a sign, two exponent bits and one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6); 32 neighbours along a row share a power of two
+``2 ** (e - 127)``, ``e`` a byte (255: the block is no number).  ``Mxfp4`` holds a matrix [rows, K], or a stack [X, rows, K]:
+
+* ``data`` uint8 [.., rows, K / 2]: number 2 i of a row in the low half of byte i, number 2 i + 1 in the high half;
+* ``scales`` uint8 [.., ceil(rows / 128), ceil(K / 128), 32, 4, 4]: the exponent of block b of row r at
+  [r // 128, b // 4, r % 32, r // 32 % 4, b % 4].  Exponents of rows and blocks past the matrix are padding, any byte but 255.
+
+``Mxfp4.from_exponents`` takes exponents row by row, ``exponents`` gives them so.
+"""
+from __future__ import annotations
+
+from contextlib import nullcontext
+from ctypes import c_float, c_int, c_longlong, c_void_p
+from typing import Optional
+
+import torch
+
+from .lib import FG_BF16, FG_F32, KernelError, check, lib, register_signatures, require_cuda, stream
+
+register_signatures("mx", {
+    "fg_mxfp4_quantize": [c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
+    "fg_mxfp4_rows": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_float, c_void_p],
+    "fg_gemm_mxfp4": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p],
+    "fg_gemm_mxfp4_grouped": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int,
+                              c_void_p],
+})
+
+BLOCK = 32
+_CODES = {torch.float32: FG_F32, torch.bfloat16: FG_BF16}
+
+
+def _scale_shape(rows: int, k: int) -> tuple:
+    return (rows + 127) // 128, (k + 127) // 128, 32, 4, 4
+
+
+class Mxfp4:
+    """A matrix [rows, k], or a stack of them, in MXFP4 (layout: the module's text)."""
+
+    __slots__ = ("data", "scales", "rows", "k")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        if data.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise KernelError(f"Mxfp4: data and scales are uint8, got {data.dtype} and {scales.dtype}")
+        shape = data.shape
+        if len(shape) not in (2, 3):
+            raise KernelError(f"Mxfp4: data is [rows, K / 2] or [X, rows, K / 2], got {tuple(shape)}")
+        self.rows, self.k = shape[-2], 2 * shape[-1]
+        if self.k == 0 or self.k % BLOCK:
+            raise KernelError(f"Mxfp4: rows of {self.k} numbers are not whole blocks of {BLOCK}")
+        want = (*shape[:-2], *_scale_shape(self.rows, self.k))
+        if scales.shape != want:
+            raise KernelError(f"Mxfp4: scales of {tuple(shape[:-1])} rows of {self.k} numbers are {want}, got {tuple(scales.shape)}")
+        if not data.is_contiguous() or not scales.is_contiguous():
+            raise KernelError("Mxfp4: data and scales must be contiguous")
+        if data.device != scales.device:
+            raise KernelError(f"Mxfp4: data is on {data.device}, scales on {scales.device}")
+        self.data, self.scales = data, scales
+
+    @property
+    def shape(self) -> tuple:
+        return (*self.data.shape[:-1], self.k)
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def __getitem__(self, i: int) -> "Mxfp4":
+        """Matrix i of a stack."""
+        if self.data.dim() != 3:
+            raise KernelError("Mxfp4: only a stack of matrices has members")
+        return Mxfp4(self.data[i], self.scales[i])
+
+    @classmethod
+    def from_exponents(cls, data: torch.Tensor, exponents: torch.Tensor) -> "Mxfp4":
+        """From exponents row by row, uint8 [.., rows, K / 32]."""
+        rows, k = data.shape[-2], 2 * data.shape[-1]
+        if exponents.dtype != torch.uint8 or k % BLOCK or exponents.shape != (*data.shape[:-1], k // BLOCK):
+            raise KernelError(f"Mxfp4: exponents are uint8 [.., rows, K / {BLOCK}], got {exponents.dtype} {tuple(exponents.shape)} for data {tuple(data.shape)}")
+        lead, n = data.shape[:-2], data.dim() - 2
+        tr, tk = _scale_shape(rows, k)[:2]
+        full = torch.zeros((*lead, tr * 128, tk * 4), dtype=torch.uint8, device=data.device)
+        full[..., :rows, :k // BLOCK] = exponents
+        full = full.reshape(*lead, tr, 4, 32, tk, 4).permute(*range(n), n, n + 3, n + 2, n + 1, n + 4)
+        return cls(data.contiguous(), full.contiguous())
+
+    def exponents(self) -> torch.Tensor:
+        """The exponents row by row, uint8 [.., rows, K / 32]."""
+        n = self.data.dim() - 2
+        tr, tk = self.scales.shape[n:n + 2]
+        full = self.scales.permute(*range(n), n, n + 3, n + 2, n + 1, n + 4).reshape(*self.data.shape[:n], tr * 128, tk * 4)
+        return full[..., :self.rows, :self.k // BLOCK].contiguous()
+
+
+def _guard(device: torch.device):
+    """Launches go to the tensors' device, whichever is current."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _same_device(what: str, device: torch.device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise KernelError(f"{what}: tensors on {device} and {t.device}")
+
+
+def _out_code(what: str, dtype: torch.dtype) -> int:
+    code = _CODES.get(dtype)
+    if code is None:
+        raise KernelError(f"{what}: cannot write {dtype}")
+    return code
+
+
+def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
+    """x [rows, K] or [X, rows, K], float32 or bfloat16, K a multiple of 32, to MXFP4.
+
+    A block's exponent is the one with which its largest number lies in [4, 8) (at least 2^-127); numbers are rounded to the nearest that the
+    format holds, ties to the even code, beyond 6 to 6.  A block that holds an infinity or no number becomes no number as a whole."""
+    require_cuda(x)
+    code = _CODES.get(x.dtype)
+    if code is None:
+        raise KernelError(f"mxfp4_quantize: rows are float32 or bfloat16, got {x.dtype}")
+    if x.dim() not in (2, 3):
+        raise KernelError(f"mxfp4_quantize: x is [rows, K] or [X, rows, K], got {tuple(x.shape)}")
+    rows, k = x.shape[-2:]
+    if k == 0 or k % BLOCK:
+        raise KernelError(f"mxfp4_quantize: rows of {k} numbers are not whole blocks of {BLOCK}")
+    if x.stride(-1) != 1:
+        raise KernelError("mxfp4_quantize: the numbers of a row must be contiguous")
+    lead = x.shape[:-2]
+    data = torch.empty((*lead, rows, k // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*lead, *_scale_shape(rows, k)), dtype=torch.uint8, device=x.device)
+    with _guard(x.device):
+        check(lib("mx").fg_mxfp4_quantize(x.data_ptr(), code, x.stride(-2), x.stride(0) if lead else 0, data.data_ptr(), scales.data_ptr(),
+                                          lead[0] if lead else 1, rows, k, stream()), "mxfp4_quantize")
+    return Mxfp4(data, scales)
+
+
+def mxfp4_rows(w: Mxfp4, rows: Optional[torch.Tensor] = None, *, scale: float = 1.0, out: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """out[i, :] = scale * w[rows[i], :] (without ``rows``: every row), float32 or bfloat16: what the matrix stands for, or the lookup in an
+    embedding table.  rows: [n] int32.  A row index outside the matrix gives a row of NaN."""
+    require_cuda(w.data, rows, out)
+    if w.data.dim() != 2:
+        raise KernelError("mxfp4_rows: w is one matrix, not a stack")
+    if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous()):
+        raise KernelError(f"mxfp4_rows: rows must be a contiguous int32 vector, got {rows.dtype} {tuple(rows.shape)}")
+    n = w.rows if rows is None else rows.numel()
+    if out is None:
+        out = torch.empty((n, w.k), dtype=out_dtype or torch.float32, device=w.device)
+    elif out.shape != (n, w.k) or out.stride(1) != 1 or (n > 1 and out.stride(0) < w.k) or (out_dtype is not None and out.dtype != out_dtype):
+        raise KernelError(f"mxfp4_rows: out must be [{n}, {w.k}] with contiguous rows")
+    code = _out_code("mxfp4_rows", out.dtype)
+    _same_device("mxfp4_rows", w.device, rows, out)
+    with _guard(w.device):
+        check(lib("mx").fg_mxfp4_rows(w.data.data_ptr(), w.scales.data_ptr(), rows.data_ptr() if rows is not None else None, out.data_ptr(), code,
+                                      max(out.stride(0), w.k), n, w.rows, w.k, float(scale), stream()), "mxfp4_rows")
+    return out
+
+
+def _output(what: str, M: int, N: int, device: torch.device, out, out_dtype, accumulate: bool) -> tuple:
+    if out is None:
+        if accumulate:
+            raise KernelError(f"{what}: accumulate needs the tensor to accumulate into")
+        out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=device)
+    elif out.shape != (M, N) or out.stride(1) != 1 or (M > 1 and out.stride(0) < N) or (out_dtype is not None and out.dtype != out_dtype):
+        raise KernelError(f"{what}: out must be [{M}, {N}] with contiguous rows")
+    code = _out_code(what, out.dtype)
+    if accumulate and code != FG_F32:
+        raise KernelError(f"{what}: the residual sum is 32-bit; accumulate needs a float32 output")
+    return out, code
+
+
+def _activations(what: str, x: torch.Tensor, k: int) -> None:
+    if x.dtype != torch.bfloat16:
+        raise KernelError(f"{what}: activations are bfloat16, got {x.dtype}")
+    if x.dim() != 2 or x.shape[1] != k:
+        raise KernelError(f"{what}: activations are [rows, {k}], got {tuple(x.shape)}")
+    if x.stride(1) != 1:
+        raise KernelError(f"{what}: the reduction dimension must be contiguous")
+
+
+def gemm_mxfp4(x: torch.Tensor, w: Mxfp4, *, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+               accumulate: bool = False) -> torch.Tensor:
+    """out[m, n] (+)= sum_k x[m, k] w[n, k]: bfloat16 activations [M, K] on a matrix [N, K] in MXFP4, float32 sums.  Output bfloat16 (default) or
+    float32; ``accumulate`` adds into a float32 ``out``."""
+    require_cuda(x, w.data, out)
+    if w.data.dim() != 2:
+        raise KernelError("gemm_mxfp4: w is one matrix, not a stack (see gemm_mxfp4_grouped)")
+    _activations("gemm_mxfp4", x, w.k)
+    M = x.shape[0]
+    out, code = _output("gemm_mxfp4", M, w.rows, x.device, out, out_dtype, accumulate)
+    _same_device("gemm_mxfp4", x.device, w.data, out)
+    with _guard(x.device):
+        check(lib("mx").fg_gemm_mxfp4(x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, out.stride(0),
+                                      int(accumulate), M, w.rows, w.k, stream()), "gemm_mxfp4")
+    return out
+
+
+def gemm_mxfp4_both(x: Mxfp4, w: Mxfp4, *, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                    accumulate: bool = False) -> torch.Tensor:
+    """The same with the activations [M, K] in MXFP4 too (``mxfp4_quantize``)."""
+    require_cuda(x.data, w.data, out)
+    if w.data.dim() != 2 or x.data.dim() != 2:
+        raise KernelError("gemm_mxfp4_both: x and w are one matrix each, not stacks")
+    if x.k != w.k:
+        raise KernelError(f"gemm_mxfp4_both: x is {x.shape} but w is {w.shape}")
+    return gemm_mxfp4(mxfp4_rows(x, out_dtype=torch.bfloat16), w, out=out, out_dtype=out_dtype, accumulate=accumulate)
+
+
+def gemm_mxfp4_grouped(x: torch.Tensor, w: Mxfp4, offsets: torch.Tensor, *, out: Optional[torch.Tensor] = None,
+                       out_dtype: Optional[torch.dtype] = None, accumulate: bool = False) -> torch.Tensor:
+    """Rows grouped by expert: out[m, n] (+)= sum_k x[m, k] w[e, n, k] for the rows offsets[e] <= m < offsets[e + 1] of expert e.
+
+    x: [M, K] bfloat16; w: a stack [X, N, K]; offsets: [X + 1] int32 on the device, rising from the first row.  Runs may be empty.  Rows of no
+    run (before the first offset, behind the last) are not written: they keep what ``out`` held, which is undefined without an ``out``."""
+    require_cuda(x, w.data, offsets, out)
+    if w.data.dim() != 3:
+        raise KernelError("gemm_mxfp4_grouped: w is a stack of matrices")
+    X = w.data.shape[0]
+    if offsets.dtype != torch.int32 or offsets.shape != (X + 1,) or not offsets.is_contiguous():
+        raise KernelError(f"gemm_mxfp4_grouped: offsets must be contiguous int32 [{X + 1}], got {offsets.dtype} {tuple(offsets.shape)}")
+    _activations("gemm_mxfp4_grouped", x, w.k)
+    M = x.shape[0]
+    out, code = _output("gemm_mxfp4_grouped", M, w.rows, x.device, out, out_dtype, accumulate)
+    _same_device("gemm_mxfp4_grouped", x.device, w.data, offsets, out)
+    with _guard(x.device):
+        check(lib("mx").fg_gemm_mxfp4_grouped(x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), offsets.data_ptr(), X, out.data_ptr(),
+                                              code, out.stride(0), int(accumulate), M, w.rows, w.k, stream()), "gemm_mxfp4_grouped")
+    return out
