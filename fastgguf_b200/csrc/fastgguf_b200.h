@@ -405,6 +405,7 @@ int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const void *scale
 /* rows offsets[e] <= m < offsets[e + 1] (device) with matrix e of a stack; rows of no run are not written */
 int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w, const void *scales, const int *offsets, int experts, void *out,
                           int out_dtype, long long ldo, int accumulate, int M, int N, int K, cudaStream_t stream);
+int fg_gemm_mxfp4_error(void);
 
 #ifdef __cplusplus
 }

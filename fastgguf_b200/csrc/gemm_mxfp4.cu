@@ -1,7 +1,7 @@
 // Contractions with weights in microscaled 4-bit floating point (format: mxfp4.cuh): out[m, n] (+)= sum_k x[m, k] w[n, k] with x in
 // bfloat16, for one matrix and for rows grouped by expert on a stack of matrices.  A weight is exact in bfloat16 and a product of two
 // bfloat16 numbers in float32; sums are float32.
-#include "mxfp4.cuh"
+#include "mxfp4_tc.cuh"
 
 struct MxGemm {
     const bf16 *x;             // [M, K], rows ldx numbers apart
@@ -20,17 +20,6 @@ __device__ __forceinline__ void mx_run(const MxGemm &a, int e, int &begin, int &
     end = min(max(a.offsets[e + 1], begin), a.M);
 }
 
-__device__ __forceinline__ void cluster_sync_all() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_dsmem_f32(uint32_t local_addr, int rank) {
-    uint32_t remote;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-    return v;
-}
 __device__ __forceinline__ void mma_bf16_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -211,6 +200,316 @@ static int launch_stream(MxGemm a, int y, cudaStream_t stream) {
     return (int)cudaLaunchKernelEx(&cfg, mxfp4_stream_kernel<NT>, a);
 }
 
+// ---------------------------------------------------------------------------- more rows: weights through tensor memory
+// A tile is 128 weight rows x BN tokens.  Weight rows are the M side of tcgen05.mma and lie in TENSOR MEMORY, where a lane is a row: a
+// thread takes 64 packed numbers of its row from shared memory, turns them into bfloat16 with their exponent in registers and stores them
+// as 32 columns (two neighbouring k a column); tokens are the N side, bfloat16 rows in shared memory as TMA brings them.  So a weight crosses
+// shared memory in its 4 bits, and the tensor core reads only the tokens there.
+//
+//   warp 0      TMA producer: stages of 128 numbers of K (tokens two boxes of 64, weights a box of 64 bytes a row, 512 bytes of exponents)
+//   warp 1      MMA issuer: eight 128 x BN x 16 a stage; its commit frees the stage, shared and tensor memory alike
+//   warps 2-9   two to a lane group of tensor memory, each half of a stage's K: unpack, and at a tile's end its epilogue.  The first
+//               stages of the next tile are unpacked BEFORE a tile's epilogue: the tensor core then goes on while results are stored.
+//
+// One CTA an SM walks the tiles; with few tiles a cluster of CTAs splits K instead, each sums a share of the columns of all partial tiles
+// out of the others' shared memory, in rank order.
+#define TILE_ROWS 128
+#define TILE_K 128
+#define TILE_THREADS 320
+#define TILE_W_BYTES (TILE_ROWS * TILE_K / 2)
+#define TILE_D_COLS 256
+#define TILE_A_COLS (TILE_K / 2)
+#define TILE_AHEAD 2            // stages of the next tile that are unpacked before a tile's epilogue
+#define TILE_MAX_EXPERTS 1024
+
+struct MxTiles {
+    MxGemm g;
+    int bn, stages, tiles_m, tiles_n, n_tiles;      // (grouped: tiles_m and n_tiles follow from the offsets)
+    int kb_per_split;
+};
+// a tile: rows [m0, m_end) of x, weight rows from n0 (row w_row of the stack, exponents from tile sc_tile)
+struct MxTile { int m0, m_end, n0, w_row, sc_tile; };
+
+__device__ __forceinline__ MxTile mx_tile(const MxTiles &a, const int *cum, int T) {
+    MxTile t;
+    if (!a.g.offsets) {
+        const int mt = T % a.tiles_m, nt = T / a.tiles_m;
+        t.m0 = mt * a.bn; t.m_end = a.g.M; t.n0 = nt * TILE_ROWS; t.w_row = t.n0; t.sc_tile = nt;
+        return t;
+    }
+    int lo = 0, hi = a.g.experts;                   // cum[e]: tiles of x in front of expert e
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cum[mid] * a.tiles_n <= T) lo = mid; else hi = mid;
+    }
+    int begin, end;
+    mx_run(a.g, lo, begin, end);
+    const int local = T - cum[lo] * a.tiles_n, tm = cum[lo + 1] - cum[lo], mt = local % tm, nt = local / tm;
+    t.m0 = begin + mt * a.bn; t.m_end = end; t.n0 = nt * TILE_ROWS; t.w_row = lo * a.g.N + t.n0; t.sc_tile = lo * a.tiles_n + nt;
+    return t;
+}
+
+__global__ void __launch_bounds__(TILE_THREADS, 1)
+mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const MxTiles a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) uint64_t bars[3 * 4 + 2];
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int cum[TILE_MAX_EXPERTS + 1];
+
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    const int bn = a.bn, stages = a.stages, S = gridDim.z, tiles_k = mx_tiles(a.g.K);
+    const int x_half = bn * 128, w_at = 2 * x_half, stage_bytes = w_at + TILE_W_BYTES + 1024;
+    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[4]), ready0 = smem_u32(&bars[8]), tfull = smem_u32(&bars[12]), tempty = smem_u32(&bars[13]);
+    const uint32_t smem0 = smem_u32(smem);
+    const int kb0 = blockIdx.z * a.kb_per_split, nkb = min(a.kb_per_split, tiles_k - kb0);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); mbar_init(ready0 + 8 * s, 8); }
+        mbar_init(tfull, 1);
+        mbar_init(tempty, 8);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tc_alloc(smem_u32(&tmem_base_s), 512);
+    int n_tiles = a.n_tiles;
+    if (a.g.offsets) {                              // tiles of x in front of each expert's run
+        if (warp == 0) {
+            int sum = 0;
+            for (int e0 = 0; e0 < a.g.experts; e0 += 32) {
+                int begin = 0, end = 0;
+                if (e0 + lane < a.g.experts) mx_run(a.g, e0 + lane, begin, end);
+                const int mine = (end - begin + bn - 1) / bn;
+                int upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+                if (e0 + lane < a.g.experts) cum[e0 + lane + 1] = sum + upto;
+                sum += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            if (lane == 0) cum[0] = 0;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+    if (a.g.offsets) n_tiles = cum[a.g.experts] * a.tiles_n;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        int s = 0, ph = 0, issued = 0;
+        bool ok = true;
+        for (int T = blockIdx.x; T < n_tiles && ok; T += gridDim.x) {
+            const MxTile t = mx_tile(a, cum, T);
+            for (int kb = kb0; kb < kb0 + nkb; kb++) {
+                ok = mbar_wait_warp(empty0 + 8 * s, ph ^ 1);
+                if (!ok) { mx_raise(1); break; }
+                if (elect_one()) {
+                    const uint32_t dst = smem0 + s * stage_bytes, bar = full0 + 8 * s;
+                    mbar_expect_tx(bar, w_at + TILE_W_BYTES + MX_TILE_BYTES);
+                    tma_load_2d(dst + w_at, &tmW, kb * (TILE_K / 2), t.w_row, bar);
+                    bulk_load(dst + w_at + TILE_W_BYTES, a.g.sc + ((size_t)t.sc_tile * tiles_k + kb) * MX_TILE_BYTES, MX_TILE_BYTES, bar);
+                    tma_load_2d(dst, &tmX, kb * TILE_K, t.m0, bar);
+                    tma_load_2d(dst + x_half, &tmX, kb * TILE_K + 64, t.m0, bar);
+                }
+                __syncwarp();
+                issued++;
+                if (++s == stages) { s = 0; ph ^= 1; }
+            }
+        }
+        for (int j = max(0, issued - stages); j < issued; j++)      // copies in flight land before the CTA exits
+            mbar_wait(full0 + 8 * (j % stages), (j / stages) & 1);
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(TILE_ROWS >> 4) << 24);
+        const uint64_t desc0 = mx_smem_desc(smem0);
+        int s = 0, ph = 0, i = 0;
+        bool ok = true;
+        for (int T = blockIdx.x; T < n_tiles && ok; T += gridDim.x, i++) {
+            if (!mbar_wait_warp(tempty, (i & 1) ^ 1)) { mx_raise(4); break; }
+            for (int kb = 0; kb < nkb; kb++) {
+                ok = mbar_wait_warp(full0 + 8 * s, ph) && mbar_wait_warp(ready0 + 8 * s, ph);
+                if (!ok) { mx_raise(2); break; }
+                tc_fence_after();
+                const uint64_t desc = desc0 + (uint64_t)(s * (stage_bytes >> 4));
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < TILE_K / 16; k++)
+                        tc_mma_bf16_ts(tmem, tmem + TILE_D_COLS + s * TILE_A_COLS + k * 8, desc + (uint64_t)((k >> 2) * (x_half >> 4) + (k & 3) * 2), idesc,
+                                       (kb | k) != 0);
+                    tc_commit(empty0 + 8 * s);
+                }
+                __syncwarp();
+                if (++s == stages) { s = 0; ph ^= 1; }
+            }
+            if (elect_one()) tc_commit(tfull);                       // also after an error: the epilogue is not left waiting
+            __syncwarp();
+        }
+    } else {
+        // ------------------------------------------------------------ unpack, epilogue
+        const int lg = warp & 3, half = (warp - 2) >> 2, r = lg * 32 + lane;
+        const uint32_t trow = tmem + ((uint32_t)(lg * 32) << 16);
+        int s = 0, ph = 0;
+        bool ok = true;
+        auto unpack = [&]() {
+            ok = mbar_wait_warp(full0 + 8 * s, ph);
+            if (!ok) { mx_raise(3); return; }
+            tc_fence_after();
+            const uint8_t *ws = smem + s * stage_bytes + w_at;
+            const uint32_t se = *(const unsigned short *)(ws + TILE_W_BYTES + lane * 16 + lg * 4 + half * 2);
+#pragma unroll
+            for (int q = 0; q < 2; q++) {                            // a block of 32 numbers
+                const uint32_t e = (se >> (8 * q)) & 255;
+                // (64 bytes a row, sixteen-byte pieces swizzled by the row)
+                const uint4 d = *(const uint4 *)(ws + r * 64 + (((half * 2 + q) ^ ((r >> 1) & 3)) << 4));
+                const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
+                const bool small = __all_sync(0xffffffffu, mx_small(e));
+                const uint32_t f = mx_factor(e);
+                uint32_t out[16];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    uint32_t v[4];
+                    mx_unpack8(dw[u], v);
+                    if (small) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) v[j] = mul_bf16x2(v[j], f);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) v[j] = mx_scale_large(v[j], e);
+                    }
+                    out[4 * u] = __byte_perm(v[0], v[1], 0x5410); out[4 * u + 1] = __byte_perm(v[2], v[3], 0x5410);
+                    out[4 * u + 2] = __byte_perm(v[0], v[1], 0x7632); out[4 * u + 3] = __byte_perm(v[2], v[3], 0x7632);
+                }
+                tc_st16(trow + TILE_D_COLS + s * TILE_A_COLS + half * 32 + q * 16, out);
+            }
+            tc_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ready0 + 8 * s);
+            if (++s == stages) { s = 0; ph ^= 1; }
+        };
+        int i = 0;
+        auto epilogue = [&](int T) {
+            const MxTile t = mx_tile(a, cum, T);
+            const bool have = mbar_wait_warp(tfull, i & 1);
+            if (!have) { mx_raise(5); ok = false; }
+            tc_fence_after();
+            uint32_t v[8][16];
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+                if ((2 * q + half) * 16 < bn) tc_ld16_async(trow + (2 * q + half) * 16, v[q]);
+            tc_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty);
+            if (S > 1) {
+                float *part = (float *)smem;                         // [bn][128]: the stages are idle
+#pragma unroll
+                for (int q = 0; q < 8; q++)
+                    if ((2 * q + half) * 16 < bn)
+#pragma unroll
+                        for (int j = 0; j < 16; j++) part[((2 * q + half) * 16 + j) * TILE_ROWS + r] = have ? __uint_as_float(v[q][j]) : 0.f;
+                return;
+            }
+            const int n = t.n0 + r;
+            if (!have || n >= a.g.N) return;
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const int m0 = t.m0 + (2 * q + half) * 16;
+                if ((2 * q + half) * 16 >= bn || m0 >= t.m_end) break;
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (m0 + j < t.m_end) mx_store(a.g, m0 + j, n, __uint_as_float(v[q][j]));
+            }
+        };
+        int before = -1;                                             // the tile whose epilogue is due
+        for (int T = blockIdx.x; T < n_tiles && ok; T += gridDim.x) {
+            int kb = 0;
+            for (; kb < min(nkb, TILE_AHEAD) && ok; kb++) unpack();
+            if (before >= 0 && ok) { epilogue(before); i++; }
+            for (; kb < nkb && ok; kb++) unpack();
+            before = T;
+        }
+        if (before >= 0) epilogue(before);
+        tc_fence_before();
+    }
+    if (S > 1) {
+        // the columns rank, rank + S, .. of the tile: partial sums of all CTAs of the cluster, in rank order
+        cluster_sync_all();
+        if (warp >= 2) {
+            const MxTile t = mx_tile(a, cum, blockIdx.x);
+            const int r = (threadIdx.x - 64) & 127, n = t.n0 + r;
+            for (int c = blockIdx.z + S * ((threadIdx.x - 64) >> 7); c < min(bn, t.m_end - t.m0); c += 2 * S) {
+                float v = 0.f;
+                for (int z = 0; z < S; z++) v += ld_dsmem_f32(smem0 + (c * TILE_ROWS + r) * 4, z);
+                if (n < a.g.N) mx_store(a.g, t.m0 + c, n, v);
+            }
+        }
+        cluster_sync_all();                                          // nobody leaves while others read its shared memory
+    }
+    __syncthreads();
+    if (warp == 1) { tc_fence_after(); tc_free(tmem, 512); }
+}
+
+static int tile_stages(int bn) {
+    const int room = 227 * 1024 - 1024 - 6 * 1024, each = bn * 256 + TILE_W_BYTES + 1024;      // (static shared memory: barriers and run lengths)
+    return room / each < 4 ? room / each : 4;
+}
+
+static int launch_tiles(const MxGemm &g, int bn, int S, int tokens_at_most, cudaStream_t stream) {
+    MxTiles a;
+    a.g = g; a.bn = bn; a.stages = tile_stages(bn);
+    const int tiles_k = mx_tiles(g.K);
+    a.tiles_n = mx_tiles(g.N); a.tiles_m = (g.M + bn - 1) / bn;
+    a.kb_per_split = (tiles_k + S - 1) / S;
+    S = (tiles_k + a.kb_per_split - 1) / a.kb_per_split;             // no CTA without a share
+    const long long tiles = (long long)(g.offsets ? (tokens_at_most + bn - 1) / bn + g.experts : a.tiles_m) * a.tiles_n;
+    if (tiles > 0x3fffffff) return FG_ERR_BAD_SIZE;
+    a.n_tiles = (int)tiles;
+    CUtensorMap tmX, tmW;
+    int rc = mx_make_map(&tmX, g.x, true, g.M, (long long)g.K * 2, g.ldx * 2, bn, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    rc = mx_make_map(&tmW, g.w, false, (long long)(g.offsets ? g.experts : 1) * g.N, g.K / 2, g.K / 2, TILE_ROWS, TILE_K / 2, CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc) return rc;
+    // All of an SM's shared memory, needed or not: a CTA that allocates tensor memory shares its SM with no other that does (of a kernel on
+    // another stream, say), whose cluster might wait for one of this kernel's while it waits for tensor memory.
+    const int smem = 227 * 1024 - 6 * 1024;
+    static FgPerDevice configured;
+    if (fg_needs_setup(configured)) {
+        cudaError_t e = cudaFuncSetAttribute(mxfp4_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return (int)e;
+    }
+    const int n_sm = mx_sm_count();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S > 1 ? (unsigned)tiles : (unsigned)(tiles < n_sm ? tiles : n_sm), 1, S);
+    cfg.blockDim = dim3(TILE_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
+    cfg.attrs = attr; cfg.numAttrs = S > 1 ? 1 : 0;
+    return (int)cudaLaunchKernelEx(&cfg, mxfp4_tile_kernel, tmX, tmW, a);
+}
+// whether TMA can bring the rows of x
+static bool tile_ok(const MxGemm &g) { return g.x_vec && g.ldx >= g.K; }
+
+// The tile's width and the split of K that finish first: rounds of tiles over the SMs times what a tile takes, in SM cycles - a stage the
+// longer of its MMAs (4 BN) and its unpacking, and once a tile its start and epilogue.
+static void tile_plan(int M, int N, int K, int n_sm, int &bn, int &S) {
+    const int tiles_k = mx_tiles(K), tiles_n = mx_tiles(N);
+    double best = 1e30;
+    for (int b = 16; b <= 256; b += 16) {
+        if (b > 16 && b - 16 >= M) break;                            // wider than the rows there are
+        const long long tiles = (long long)((M + b - 1) / b) * tiles_n;
+        for (int s = 1; s <= 8; s++) {
+            if (s > 1 && tiles * s > n_sm) break;
+            const int kb = (tiles_k + s - 1) / s;
+            const double stage = 4.0 * b > 450 ? 4.0 * b : 450;
+            const double tile = kb * stage + 1500 + 6.0 * b + (s > 1 ? 1500 + 12.0 * b : 0);
+            const double cost = (double)((tiles * s + n_sm - 1) / n_sm) * tile;
+            if (cost < best) { best = cost; bn = b; S = s; }
+        }
+    }
+}
+
 static int mx_check(const MxGemm &a) {
     if (a.out_dtype != FG_F32 && a.out_dtype != FG_BF16) return FG_ERR_BAD_DTYPE;
     if (a.accumulate && a.out_dtype != FG_F32) return FG_ERR_BAD_DTYPE;
@@ -226,6 +525,11 @@ extern "C" int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const 
     if (M == 0) return 0;
     a.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     if (M <= 8) return launch_stream<1>(a, 1, stream);
+    if (M > 16 && tile_ok(a)) {
+        int bn, S;
+        tile_plan(M, N, K, mx_sm_count(), bn, S);
+        return launch_tiles(a, bn, S, M, stream);
+    }
     if (M > 65535 * 16) return FG_ERR_BAD_SIZE;
     return launch_stream<2>(a, (M + 15) / 16, stream);
 }
@@ -239,5 +543,14 @@ extern "C" int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w
     if (experts <= 0 || experts > 65535 || !offsets) return FG_ERR_BAD_SIZE;
     if (M == 0) return 0;
     a.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
+    if (M > 16ll * experts && experts <= TILE_MAX_EXPERTS && tile_ok(a)) return launch_tiles(a, 128, 1, M, stream);
     return (long long)M <= 4ll * experts ? launch_stream<1>(a, experts, stream) : launch_stream<2>(a, experts, stream);
+}
+
+// 0, or (code << 8 | role) of the first bounded wait that ran out since it was asked last
+extern "C" int fg_gemm_mxfp4_error(void) {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_mx_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_mx_error, &zero, sizeof(int));
+    return v;
 }

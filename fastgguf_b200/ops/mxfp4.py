@@ -26,6 +26,7 @@ register_signatures("mx", {
     "fg_gemm_mxfp4": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p],
     "fg_gemm_mxfp4_grouped": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int,
                               c_void_p],
+    "fg_gemm_mxfp4_error": [],
 })
 
 BLOCK = 32
