@@ -402,6 +402,10 @@ int fg_mxfp4_rows(const void *data, const void *scales, const int *rows, void *o
 /* out (+)= x w^T: x [M, K] bfloat16, w [N, K]; out bfloat16 or float32, accumulate: float32 alone */
 int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
                   int M, int N, int K, cudaStream_t stream);
+/* the same with the kernel named: form 0 by the rule, 1 for few rows, 2 tiles, 3 tiles of pairs of CTAs; bn tokens a tile (a multiple of 16,
+   up to 256), K over `splits` CTAs (form 2, up to 8) */
+int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
+                      int M, int N, int K, int form, int bn, int splits, cudaStream_t stream);
 /* rows offsets[e] <= m < offsets[e + 1] (device) with matrix e of a stack; rows of no run are not written */
 int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w, const void *scales, const int *offsets, int experts, void *out,
                           int out_dtype, long long ldo, int accumulate, int M, int N, int K, cudaStream_t stream);

@@ -122,13 +122,13 @@ mxfp4_stream_kernel(MxGemm a) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         mx_unpack8(u == 0 ? cur[j].x : u == 1 ? cur[j].y : u == 2 ? cur[j].z : cur[j].w, r[j]);
-                        if (small) {
-                            const uint32_t f = mx_factor(se[j]);
+                        const uint32_t f = mx_factor(se[j]);
 #pragma unroll
-                            for (int q = 0; q < 4; q++) r[j][q] = mul_bf16x2(r[j][q], f);
-                        } else {
+                        for (int q = 0; q < 4; q++) r[j][q] = mul_bf16x2(r[j][q], f);
+                        if (!small) {
+                            const uint32_t rest = mx_factor_rest(se[j]);
 #pragma unroll
-                            for (int q = 0; q < 4; q++) r[j][q] = mx_scale_large(r[j][q], se[j]);
+                            for (int q = 0; q < 4; q++) r[j][q] = mul_bf16x2(r[j][q], rest);
                         }
                     }
 #pragma unroll
@@ -202,310 +202,363 @@ static int launch_stream(MxGemm a, int y, cudaStream_t stream) {
 
 // ---------------------------------------------------------------------------- more rows: weights through tensor memory
 // A tile is 128 weight rows x BN tokens.  Weight rows are the M side of tcgen05.mma and lie in TENSOR MEMORY, where a lane is a row: a
-// thread takes 64 packed numbers of its row from shared memory, turns them into bfloat16 with their exponent in registers and stores them
-// as 32 columns (two neighbouring k a column); tokens are the N side, bfloat16 rows in shared memory as TMA brings them.  So a weight crosses
-// shared memory in its 4 bits, and the tensor core reads only the tokens there.
+// thread takes 64 packed numbers of its row from shared memory, turns them into bfloat16 with their exponents in registers and stores them
+// as 32 columns (two neighbouring k a column); tokens are the N side, bfloat16 rows in shared memory as TMA brings them.  So a weight
+// crosses shared memory in its 4 bits, and the tensor core reads only the tokens there.  K goes in stages of 128.
 //
-//   warp 0      TMA producer: stages of 128 numbers of K (tokens two boxes of 64, weights a box of 64 bytes a row, 512 bytes of exponents)
-//   warp 1      MMA issuer: eight 128 x BN x 16 a stage; its commit frees the stage, shared and tensor memory alike
-//   warps 2-9   two to a lane group of tensor memory, each half of a stage's K: unpack, and at a tile's end its epilogue.  The first
-//               stages of the next tile are unpacked BEFORE a tile's epilogue: the tensor core then goes on while results are stored.
+//   warp 0      tokens: two boxes of 64 numbers a stage, a ring of up to four
+//   warp 1      MMA issuer: eight 128 x BN x 16 a stage; its commit frees the stage's tokens and its slot of tensor memory (four of 64 columns)
+//   warp 2      weights: 64 bytes a row and 512 bytes of exponents a stage, a ring of six
+//   warps 3-18  four to a lane group of tensor memory, for the halves of the even and of the odd stages: unpack, and at a tile's end its
+//               epilogue.  The first stages of the next tile are unpacked BEFORE a tile's epilogue: the tensor core goes on meanwhile.
+// A stage's unpacking takes a warp about 1,100 cycles from its wait for the weights to its arrival, most of it latency, and a stage's MMAs
+// 1,024 at 256 tokens: two warps a scheduler do not keep up (2,048 x 8,192 x 4,096: 133 us), four do.
 //
-// One CTA an SM walks the tiles; with few tiles a cluster of CTAs splits K instead, each sums a share of the columns of all partial tiles
-// out of the others' shared memory, in rank order.
+// One CTA an SM walks the tiles.  PAIR: two CTAs of a cluster take 256 weight rows x BN tokens (tcgen05.mma.cta_group::2); each unpacks its
+// own 128 rows and brings half of the tokens, which halves the bytes an SM receives per MMA.  With few tiles a cluster of single CTAs splits
+// K instead; each sums a share of the columns of all partial tiles out of the others' shared memory, in rank order.
 #define TILE_ROWS 128
 #define TILE_K 128
-#define TILE_THREADS 320
+#define TILE_THREADS 608
 #define TILE_W_BYTES (TILE_ROWS * TILE_K / 2)
-#define TILE_D_COLS 256
-#define TILE_A_COLS (TILE_K / 2)
-#define TILE_AHEAD 2            // stages of the next tile that are unpacked before a tile's epilogue
+#define TILE_W_STAGE (TILE_W_BYTES + 1024)
+#define TILE_W_STAGES 6
+#define TILE_SLOTS 4            // stages in tensor memory, 64 columns each, behind the accumulator's 256
+#define TILE_AHEAD 3            // stages of the next tile that are unpacked before a tile's epilogue
 #define TILE_MAX_EXPERTS 1024
+#define TILE_SMEM (221 * 1024)
+#define TILE_UNPACK 520         // SM cycles that unpacking a stage takes at least (the integer pipe's)
 
 struct MxTiles {
     MxGemm g;
-    int bn, stages, tiles_m, tiles_n, n_tiles;      // (grouped: tiles_m and n_tiles follow from the offsets)
+    int bn, xs, tiles_m, tiles_n, n_tiles;          // tokens a tile, depth of their ring (grouped: tiles_m and n_tiles follow from the offsets)
     int kb_per_split;
 };
 // a tile: rows [m0, m_end) of x, weight rows from n0 (row w_row of the stack, exponents from tile sc_tile)
 struct MxTile { int m0, m_end, n0, w_row, sc_tile; };
 
-__device__ __forceinline__ MxTile mx_tile(const MxTiles &a, const int *cum, int T) {
+template <bool PAIR>
+__device__ __forceinline__ MxTile mx_tile(const MxTiles &a, const int *cum, int T, int rank) {
     MxTile t;
+    int nt, e = 0;
     if (!a.g.offsets) {
-        const int mt = T % a.tiles_m, nt = T / a.tiles_m;
-        t.m0 = mt * a.bn; t.m_end = a.g.M; t.n0 = nt * TILE_ROWS; t.w_row = t.n0; t.sc_tile = nt;
-        return t;
+        t.m0 = T % a.tiles_m * a.bn; t.m_end = a.g.M; nt = T / a.tiles_m;
+    } else {
+        int hi = a.g.experts;                       // cum[e]: tiles of x in front of expert e
+        while (hi - e > 1) {
+            const int mid = (e + hi) >> 1;
+            if (cum[mid] * a.tiles_n <= T) e = mid; else hi = mid;
+        }
+        int begin, end;
+        mx_run(a.g, e, begin, end);
+        const int local = T - cum[e] * a.tiles_n, tm = cum[e + 1] - cum[e];
+        t.m0 = begin + local % tm * a.bn; t.m_end = end; nt = local / tm;
     }
-    int lo = 0, hi = a.g.experts;                   // cum[e]: tiles of x in front of expert e
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cum[mid] * a.tiles_n <= T) lo = mid; else hi = mid;
-    }
-    int begin, end;
-    mx_run(a.g, lo, begin, end);
-    const int local = T - cum[lo] * a.tiles_n, tm = cum[lo + 1] - cum[lo], mt = local % tm, nt = local / tm;
-    t.m0 = begin + mt * a.bn; t.m_end = end; t.n0 = nt * TILE_ROWS; t.w_row = lo * a.g.N + t.n0; t.sc_tile = lo * a.tiles_n + nt;
+    const int n128 = PAIR ? 2 * nt + rank : nt, all128 = mx_tiles(a.g.N);
+    t.n0 = n128 * TILE_ROWS;
+    t.w_row = e * a.g.N + t.n0;
+    t.sc_tile = e * all128 + min(n128, all128 - 1);     // (a pair's second half may lie past the matrix: its rows are not stored)
     return t;
 }
 
+// Sixteen columns (tokens m0 ..) of this thread's weight row n
+__device__ __forceinline__ void tile_store(const MxGemm &a, int m0, int m_end, int n, const uint32_t (&v)[16]) {
+    const int count = min(16, m_end - m0);
+    const size_t at = (size_t)m0 * a.ldo + n;
+    if (a.out_dtype == FG_BF16) {
+        bf16 *o = (bf16 *)a.out + at;
+#pragma unroll
+        for (int j = 0; j < 16; j++, o += a.ldo)
+            if (j < count) *o = __float2bfloat16_rn(__uint_as_float(v[j]));
+    } else if (a.accumulate) {
+        float *o = (float *)a.out + at;
+#pragma unroll
+        for (int j = 0; j < 16; j++, o += a.ldo)
+            if (j < count) *o += __uint_as_float(v[j]);
+    } else {
+        float *o = (float *)a.out + at;
+#pragma unroll
+        for (int j = 0; j < 16; j++, o += a.ldo)
+            if (j < count) *o = __uint_as_float(v[j]);
+    }
+}
+
+template <bool PAIR>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
 mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const MxTiles a) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t bars[3 * 4 + 2];
+    __shared__ __align__(8) uint64_t bars[2 * TILE_W_STAGES + 2 * TILE_SLOTS + 2];
     __shared__ uint32_t tmem_base_s;
     __shared__ int cum[TILE_MAX_EXPERTS + 1];
 
     const int warp = warp_index(), lane = threadIdx.x & 31;
-    const int bn = a.bn, stages = a.stages, S = gridDim.z, tiles_k = mx_tiles(a.g.K);
-    const int x_half = bn * 128, w_at = 2 * x_half, stage_bytes = w_at + TILE_W_BYTES + 1024;
-    const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[4]), ready0 = smem_u32(&bars[8]), tfull = smem_u32(&bars[12]), tempty = smem_u32(&bars[13]);
+    const int bn = a.bn, xs = a.xs, S = gridDim.z, tiles_k = mx_tiles(a.g.K);
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0, first = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, stride = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+    const int x_half = (PAIR ? bn / 2 : bn) * 128, x_bytes = 2 * x_half;
+    // full[slot]: a stage's weights are in tensor memory (eight warps a CTA) and its tokens in shared memory; done[slot]: its MMAs are complete
+    const uint32_t wfull0 = smem_u32(&bars[0]), wempty0 = wfull0 + 8 * TILE_W_STAGES, full0 = wempty0 + 8 * TILE_W_STAGES, done0 = full0 + 8 * TILE_SLOTS,
+                   tfull = done0 + 8 * TILE_SLOTS, tempty = tfull + 8;
     const uint32_t smem0 = smem_u32(smem);
+    uint8_t *wring = smem + xs * x_bytes;
     const int kb0 = blockIdx.z * a.kb_per_split, nkb = min(a.kb_per_split, tiles_k - kb0);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); mbar_init(ready0 + 8 * s, 8); }
+        for (int s = 0; s < TILE_W_STAGES; s++) { mbar_init(wfull0 + 8 * s, 1); mbar_init(wempty0 + 8 * s, 8); }
+        for (int s = 0; s < TILE_SLOTS; s++) { mbar_init(full0 + 8 * s, PAIR ? 17 : 9); mbar_init(done0 + 8 * s, 1); }
         mbar_init(tfull, 1);
-        mbar_init(tempty, 8);
+        mbar_init(tempty, PAIR ? 32 : 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tc_alloc(smem_u32(&tmem_base_s), 512);
-    int n_tiles = a.n_tiles;
-    if (a.g.offsets) {                              // tiles of x in front of each expert's run
-        if (warp == 0) {
-            int sum = 0;
-            for (int e0 = 0; e0 < a.g.experts; e0 += 32) {
-                int begin = 0, end = 0;
-                if (e0 + lane < a.g.experts) mx_run(a.g, e0 + lane, begin, end);
-                const int mine = (end - begin + bn - 1) / bn;
-                int upto = mine;
+    if (warp == 1) { if (PAIR) tc_alloc_pair(smem_u32(&tmem_base_s), 512); else tc_alloc(smem_u32(&tmem_base_s), 512); }
+    if (a.g.offsets && warp == 0) {                 // tiles of x in front of each expert's run
+        int sum = 0;
+        for (int e0 = 0; e0 < a.g.experts; e0 += 32) {
+            int begin = 0, end = 0;
+            if (e0 + lane < a.g.experts) mx_run(a.g, e0 + lane, begin, end);
+            int upto = (end - begin + bn - 1) / bn;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
-                if (e0 + lane < a.g.experts) cum[e0 + lane + 1] = sum + upto;
-                sum += __shfl_sync(0xffffffffu, upto, 31);
-            }
-            if (lane == 0) cum[0] = 0;
+            for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+            if (e0 + lane < a.g.experts) cum[e0 + lane + 1] = sum + upto;
+            sum += __shfl_sync(0xffffffffu, upto, 31);
         }
+        if (lane == 0) cum[0] = 0;
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync_all();                   // the partner's barriers exist before anything arrives on them
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;
-    if (a.g.offsets) n_tiles = cum[a.g.experts] * a.tiles_n;
+    const int n_tiles = a.g.offsets ? cum[a.g.experts] * a.tiles_n : a.n_tiles;
 
     if (warp == 0) {
-        // ------------------------------------------------------------ TMA producer
-        int s = 0, ph = 0, issued = 0;
+        // ------------------------------------------------------------ tokens (both CTAs of a pair; they complete on the leader's barriers)
+        const uint32_t full = PAIR ? mapa_u32(full0, 0) : full0;
+        int g = 0, s = 0;
         bool ok = true;
-        for (int T = blockIdx.x; T < n_tiles && ok; T += gridDim.x) {
-            const MxTile t = mx_tile(a, cum, T);
-            for (int kb = kb0; kb < kb0 + nkb; kb++) {
-                ok = mbar_wait_warp(empty0 + 8 * s, ph ^ 1);
+        for (int T = first; T < n_tiles && ok; T += stride) {
+            const int m0 = mx_tile<PAIR>(a, cum, T, rank).m0 + (PAIR ? rank * (bn / 2) : 0);
+            for (int kb = kb0; kb < kb0 + nkb; kb++, g++) {
+                const int was = g - xs, slot = g % TILE_SLOTS;      // `was`: the stage that used this place before
+                if (was >= 0) ok = mbar_wait_warp(done0 + 8 * (was % TILE_SLOTS), (was / TILE_SLOTS) & 1);
                 if (!ok) { mx_raise(1); break; }
                 if (elect_one()) {
-                    const uint32_t dst = smem0 + s * stage_bytes, bar = full0 + 8 * s;
-                    mbar_expect_tx(bar, w_at + TILE_W_BYTES + MX_TILE_BYTES);
-                    tma_load_2d(dst + w_at, &tmW, kb * (TILE_K / 2), t.w_row, bar);
-                    bulk_load(dst + w_at + TILE_W_BYTES, a.g.sc + ((size_t)t.sc_tile * tiles_k + kb) * MX_TILE_BYTES, MX_TILE_BYTES, bar);
-                    tma_load_2d(dst, &tmX, kb * TILE_K, t.m0, bar);
-                    tma_load_2d(dst + x_half, &tmX, kb * TILE_K + 64, t.m0, bar);
+                    const uint32_t dst = smem0 + s * x_bytes, bar = full + 8 * slot;
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * slot, (PAIR ? 2 : 1) * x_bytes);
+                    if (PAIR) { tma_load_2d_pair(dst, &tmX, kb * TILE_K, m0, bar); tma_load_2d_pair(dst + x_half, &tmX, kb * TILE_K + 64, m0, bar); }
+                    else { tma_load_2d(dst, &tmX, kb * TILE_K, m0, bar); tma_load_2d(dst + x_half, &tmX, kb * TILE_K + 64, m0, bar); }
                 }
                 __syncwarp();
-                issued++;
-                if (++s == stages) { s = 0; ph ^= 1; }
+                if (++s == xs) s = 0;
             }
         }
-        for (int j = max(0, issued - stages); j < issued; j++)      // copies in flight land before the CTA exits
-            mbar_wait(full0 + 8 * (j % stages), (j / stages) & 1);
+        if (rank == 0)                              // copies in flight land before the CTA exits
+            for (int j = max(0, g - xs); j < g; j++) mbar_wait(full0 + 8 * (j % TILE_SLOTS), (j / TILE_SLOTS) & 1);
     } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer
-        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(TILE_ROWS >> 4) << 24);
+        // ------------------------------------------------------------ MMA issuer (a pair's leader alone)
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)((PAIR ? 2 : 1) * TILE_ROWS >> 4) << 24);
         const uint64_t desc0 = mx_smem_desc(smem0);
-        int s = 0, ph = 0, i = 0;
-        bool ok = true;
-        for (int T = blockIdx.x; T < n_tiles && ok; T += gridDim.x, i++) {
-            if (!mbar_wait_warp(tempty, (i & 1) ^ 1)) { mx_raise(4); break; }
-            for (int kb = 0; kb < nkb; kb++) {
-                ok = mbar_wait_warp(full0 + 8 * s, ph) && mbar_wait_warp(ready0 + 8 * s, ph);
+        int g = 0, s = 0, i = 0;
+        bool ok = rank == 0;
+        for (int T = first; T < n_tiles && ok; T += stride, i++) {
+            ok = mbar_wait_warp(tempty, (i & 1) ^ 1);
+            if (!ok) { mx_raise(4); break; }
+            for (int kb = 0; kb < nkb; kb++, g++) {
+                const int slot = g % TILE_SLOTS;
+                ok = mbar_wait_warp(full0 + 8 * slot, (g / TILE_SLOTS) & 1);
                 if (!ok) { mx_raise(2); break; }
                 tc_fence_after();
-                const uint64_t desc = desc0 + (uint64_t)(s * (stage_bytes >> 4));
+                const uint64_t desc = desc0 + (uint64_t)(s * (x_bytes >> 4));
+                const uint32_t at = tmem + 256 + slot * 64;
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < TILE_K / 16; k++)
-                        tc_mma_bf16_ts(tmem, tmem + TILE_D_COLS + s * TILE_A_COLS + k * 8, desc + (uint64_t)((k >> 2) * (x_half >> 4) + (k & 3) * 2), idesc,
-                                       (kb | k) != 0);
-                    tc_commit(empty0 + 8 * s);
+                    for (int k = 0; k < 8; k++) {
+                        const uint64_t d = desc + (uint64_t)((k >> 2) * (x_half >> 4) + (k & 3) * 2);
+                        if (PAIR) tc_mma_bf16_ts_pair(tmem, at + k * 8, d, idesc, (kb | k) != 0);
+                        else tc_mma_bf16_ts(tmem, at + k * 8, d, idesc, (kb | k) != 0);
+                    }
+                    if (PAIR) tc_commit_pair(done0 + 8 * slot); else tc_commit(done0 + 8 * slot);
                 }
                 __syncwarp();
-                if (++s == stages) { s = 0; ph ^= 1; }
+                if (++s == xs) s = 0;
             }
-            if (elect_one()) tc_commit(tfull);                       // also after an error: the epilogue is not left waiting
+            if (elect_one()) { if (PAIR) tc_commit_pair(tfull); else tc_commit(tfull); }      // also after an error: the epilogue is not left waiting
             __syncwarp();
         }
+    } else if (warp == 2) {
+        // ------------------------------------------------------------ weights and exponents
+        int s = 0, ph = 0, issued = 0;
+        bool ok = true;
+        const uint32_t ring = smem_u32(wring);
+        for (int T = first; T < n_tiles && ok; T += stride) {
+            const MxTile t = mx_tile<PAIR>(a, cum, T, rank);
+            for (int kb = kb0; kb < kb0 + nkb; kb++, issued++) {
+                ok = mbar_wait_warp(wempty0 + 8 * s, ph ^ 1);
+                if (!ok) { mx_raise(6); break; }
+                if (elect_one()) {
+                    const uint32_t dst = ring + s * TILE_W_STAGE, bar = wfull0 + 8 * s;
+                    mbar_expect_tx(bar, TILE_W_BYTES + MX_TILE_BYTES);
+                    tma_load_2d(dst, &tmW, kb * (TILE_K / 2), t.w_row, bar);
+                    bulk_load(dst + TILE_W_BYTES, a.g.sc + ((size_t)t.sc_tile * tiles_k + kb) * MX_TILE_BYTES, MX_TILE_BYTES, bar);
+                }
+                __syncwarp();
+                if (++s == TILE_W_STAGES) { s = 0; ph ^= 1; }
+            }
+        }
+        for (int j = max(0, issued - TILE_W_STAGES); j < issued; j++) mbar_wait(wfull0 + 8 * (j % TILE_W_STAGES), (j / TILE_W_STAGES) & 1);
     } else {
         // ------------------------------------------------------------ unpack, epilogue
-        const int lg = warp & 3, half = (warp - 2) >> 2, r = lg * 32 + lane;
+        const int lg = warp & 3, set = (warp - 3) >> 2, half = set & 1, parity = set >> 1, r = lg * 32 + lane;
         const uint32_t trow = tmem + ((uint32_t)(lg * 32) << 16);
-        int s = 0, ph = 0;
+        const uint32_t full = PAIR ? mapa_u32(full0, 0) : full0, empty = PAIR ? mapa_u32(tempty, 0) : tempty;
+        int g = 0, i = 0;                           // the stage this tile starts with, tiles finished
         bool ok = true;
-        auto unpack = [&]() {
-            ok = mbar_wait_warp(full0 + 8 * s, ph);
+        auto unpack = [&](int stage) {
+            const int s = stage % TILE_W_STAGES, slot = stage % TILE_SLOTS;
+            ok = mbar_wait_warp(wfull0 + 8 * s, (stage / TILE_W_STAGES) & 1);
             if (!ok) { mx_raise(3); return; }
-            tc_fence_after();
-            const uint8_t *ws = smem + s * stage_bytes + w_at;
+            const uint8_t *ws = wring + s * TILE_W_STAGE;
             const uint32_t se = *(const unsigned short *)(ws + TILE_W_BYTES + lane * 16 + lg * 4 + half * 2);
+            uint4 d[2];                             // (64 bytes a row, sixteen-byte pieces swizzled by the row)
 #pragma unroll
-            for (int q = 0; q < 2; q++) {                            // a block of 32 numbers
-                const uint32_t e = (se >> (8 * q)) & 255;
-                // (64 bytes a row, sixteen-byte pieces swizzled by the row)
-                const uint4 d = *(const uint4 *)(ws + r * 64 + (((half * 2 + q) ^ ((r >> 1) & 3)) << 4));
-                const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
-                const bool small = __all_sync(0xffffffffu, mx_small(e));
-                const uint32_t f = mx_factor(e);
+            for (int q = 0; q < 2; q++) d[q] = *(const uint4 *)(ws + r * 64 + (((half * 2 + q) ^ ((r >> 1) & 3)) << 4));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(wempty0 + 8 * s);
+            if (stage >= TILE_SLOTS) {
+                ok = mbar_wait_warp(done0 + 8 * slot, (stage / TILE_SLOTS - 1) & 1);
+                if (!ok) { mx_raise(7); return; }
+            }
+            tc_fence_after();
+            const uint32_t at = trow + 256 + slot * 64 + half * 32;
+#pragma unroll
+            for (int q = 0; q < 2; q++) {           // a block of 32 numbers
                 uint32_t out[16];
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    uint32_t v[4];
-                    mx_unpack8(dw[u], v);
-                    if (small) {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) v[j] = mul_bf16x2(v[j], f);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) v[j] = mx_scale_large(v[j], e);
-                    }
-                    out[4 * u] = __byte_perm(v[0], v[1], 0x5410); out[4 * u + 1] = __byte_perm(v[2], v[3], 0x5410);
-                    out[4 * u + 2] = __byte_perm(v[0], v[1], 0x7632); out[4 * u + 3] = __byte_perm(v[2], v[3], 0x7632);
-                }
-                tc_st16(trow + TILE_D_COLS + s * TILE_A_COLS + half * 32 + q * 16, out);
+                mx_unpack32(d[q], (se >> (8 * q)) & 255, out);
+                tc_st16(at + q * 16, out);
             }
             tc_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(ready0 + 8 * s);
-            if (++s == stages) { s = 0; ph ^= 1; }
+            if (lane == 0) { if (PAIR) mbar_arrive_cluster(full + 8 * slot); else mbar_arrive(full + 8 * slot); }
         };
-        int i = 0;
         auto epilogue = [&](int T) {
-            const MxTile t = mx_tile(a, cum, T);
+            const MxTile t = mx_tile<PAIR>(a, cum, T, rank);
             const bool have = mbar_wait_warp(tfull, i & 1);
             if (!have) { mx_raise(5); ok = false; }
             tc_fence_after();
-            uint32_t v[8][16];
+            uint32_t v[4][16];                      // columns 16 (4 q + set) ..
 #pragma unroll
-            for (int q = 0; q < 8; q++)
-                if ((2 * q + half) * 16 < bn) tc_ld16_async(trow + (2 * q + half) * 16, v[q]);
+            for (int q = 0; q < 4; q++)
+                if ((4 * q + set) * 16 < bn) tc_ld16_async(trow + (4 * q + set) * 16, v[q]);
             tc_ld_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(tempty);
-            if (S > 1) {
-                float *part = (float *)smem;                         // [bn][128]: the stages are idle
+            if (lane == 0) { if (PAIR) mbar_arrive_cluster(empty); else mbar_arrive(empty); }
+            if (!PAIR && S > 1) {
+                float *part = (float *)smem;        // [bn][128]: the rings are idle
 #pragma unroll
-                for (int q = 0; q < 8; q++)
-                    if ((2 * q + half) * 16 < bn)
+                for (int q = 0; q < 4; q++)
+                    if ((4 * q + set) * 16 < bn)
 #pragma unroll
-                        for (int j = 0; j < 16; j++) part[((2 * q + half) * 16 + j) * TILE_ROWS + r] = have ? __uint_as_float(v[q][j]) : 0.f;
+                        for (int j = 0; j < 16; j++) part[((4 * q + set) * 16 + j) * TILE_ROWS + r] = have ? __uint_as_float(v[q][j]) : 0.f;
                 return;
             }
             const int n = t.n0 + r;
             if (!have || n >= a.g.N) return;
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
-                const int m0 = t.m0 + (2 * q + half) * 16;
-                if ((2 * q + half) * 16 >= bn || m0 >= t.m_end) break;
-#pragma unroll
-                for (int j = 0; j < 16; j++)
-                    if (m0 + j < t.m_end) mx_store(a.g, m0 + j, n, __uint_as_float(v[q][j]));
-            }
+            for (int q = 0; q < 4; q++)
+                if ((4 * q + set) * 16 < bn) tile_store(a.g, t.m0 + (4 * q + set) * 16, t.m_end, n, v[q]);
         };
-        int before = -1;                                             // the tile whose epilogue is due
-        for (int T = blockIdx.x; T < n_tiles && ok; T += gridDim.x) {
-            int kb = 0;
-            for (; kb < min(nkb, TILE_AHEAD) && ok; kb++) unpack();
-            if (before >= 0 && ok) { epilogue(before); i++; }
-            for (; kb < nkb && ok; kb++) unpack();
-            before = T;
+        // (one loop, so that the code of each stands once: the epilogue of the tile `before` comes behind the first stages of the next)
+        for (int T = first, before = -1; ; before = T, T += stride) {
+            const int stages = T < n_tiles && ok ? nkb : 0, lead = min(stages, TILE_AHEAD);
+            for (int kb = 0; kb <= stages; kb++) {
+                if (kb == lead && before >= 0) { epilogue(before); i++; }
+                if (kb < stages && ok && ((g + kb) & 1) == parity) unpack(g + kb);
+            }
+            if (stages == 0) break;
+            g += stages;
         }
-        if (before >= 0) epilogue(before);
         tc_fence_before();
     }
-    if (S > 1) {
+    if (!PAIR && S > 1) {
         // the columns rank, rank + S, .. of the tile: partial sums of all CTAs of the cluster, in rank order
         cluster_sync_all();
-        if (warp >= 2) {
-            const MxTile t = mx_tile(a, cum, blockIdx.x);
-            const int r = (threadIdx.x - 64) & 127, n = t.n0 + r;
-            for (int c = blockIdx.z + S * ((threadIdx.x - 64) >> 7); c < min(bn, t.m_end - t.m0); c += 2 * S) {
+        if (warp >= 3) {
+            const MxTile t = mx_tile<PAIR>(a, cum, first, rank);
+            const int r = (threadIdx.x - 96) & 127, n = t.n0 + r;
+            for (int c = blockIdx.z + S * ((threadIdx.x - 96) >> 7); c < min(bn, t.m_end - t.m0); c += 4 * S) {
                 float v = 0.f;
                 for (int z = 0; z < S; z++) v += ld_dsmem_f32(smem0 + (c * TILE_ROWS + r) * 4, z);
                 if (n < a.g.N) mx_store(a.g, t.m0 + c, n, v);
             }
         }
-        cluster_sync_all();                                          // nobody leaves while others read its shared memory
+        cluster_sync_all();                         // nobody leaves while others read its shared memory
     }
+    tc_fence_before();
     __syncthreads();
-    if (warp == 1) { tc_fence_after(); tc_free(tmem, 512); }
+    // neither CTA of a pair leaves, or frees tensor memory, while the other's copies complete on its barriers or the MMAs read its memory
+    if (PAIR) cluster_sync_all();
+    if (warp == 1) { tc_fence_after(); if (PAIR) tc_free_pair(tmem, 512); else tc_free(tmem, 512); }
 }
 
-static int tile_stages(int bn) {
-    const int room = 227 * 1024 - 1024 - 6 * 1024, each = bn * 256 + TILE_W_BYTES + 1024;      // (static shared memory: barriers and run lengths)
-    return room / each < 4 ? room / each : 4;
-}
-
-static int launch_tiles(const MxGemm &g, int bn, int S, int tokens_at_most, cudaStream_t stream) {
+template <bool PAIR>
+static int launch_tiles(const MxGemm &g, int bn, int S, cudaStream_t stream) {
     MxTiles a;
-    a.g = g; a.bn = bn; a.stages = tile_stages(bn);
-    const int tiles_k = mx_tiles(g.K);
-    a.tiles_n = mx_tiles(g.N); a.tiles_m = (g.M + bn - 1) / bn;
+    a.g = g; a.bn = bn;
+    const int x_bytes = (PAIR ? bn / 2 : bn) * 256, room = (TILE_SMEM - 1024 - TILE_W_STAGES * TILE_W_STAGE) / x_bytes;
+    a.xs = room < TILE_SLOTS ? room : TILE_SLOTS;
+    const int tiles_k = mx_tiles(g.K), rows = PAIR ? 2 * TILE_ROWS : TILE_ROWS;
+    a.tiles_n = (g.N + rows - 1) / rows; a.tiles_m = (g.M + bn - 1) / bn;
     a.kb_per_split = (tiles_k + S - 1) / S;
     S = (tiles_k + a.kb_per_split - 1) / a.kb_per_split;             // no CTA without a share
-    const long long tiles = (long long)(g.offsets ? (tokens_at_most + bn - 1) / bn + g.experts : a.tiles_m) * a.tiles_n;
+    const long long tiles = (long long)(g.offsets ? a.tiles_m + g.experts : a.tiles_m) * a.tiles_n;
     if (tiles > 0x3fffffff) return FG_ERR_BAD_SIZE;
     a.n_tiles = (int)tiles;
     CUtensorMap tmX, tmW;
-    int rc = mx_make_map(&tmX, g.x, true, g.M, (long long)g.K * 2, g.ldx * 2, bn, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = mx_make_map(&tmX, g.x, true, g.M, (long long)g.K * 2, g.ldx * 2, PAIR ? bn / 2 : bn, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     rc = mx_make_map(&tmW, g.w, false, (long long)(g.offsets ? g.experts : 1) * g.N, g.K / 2, g.K / 2, TILE_ROWS, TILE_K / 2, CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc) return rc;
     // All of an SM's shared memory, needed or not: a CTA that allocates tensor memory shares its SM with no other that does (of a kernel on
     // another stream, say), whose cluster might wait for one of this kernel's while it waits for tensor memory.
-    const int smem = 227 * 1024 - 6 * 1024;
     static FgPerDevice configured;
     if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(mxfp4_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaError_t e = cudaFuncSetAttribute(mxfp4_tile_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM);
         if (e != cudaSuccess) return (int)e;
     }
-    const int n_sm = mx_sm_count();
+    const int units = PAIR ? mx_sm_count() / 2 : mx_sm_count();
+    const unsigned gx = S > 1 || tiles < units ? (unsigned)tiles : (unsigned)units;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(S > 1 ? (unsigned)tiles : (unsigned)(tiles < n_sm ? tiles : n_sm), 1, S);
-    cfg.blockDim = dim3(TILE_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cfg.gridDim = dim3(PAIR ? 2 * gx : gx, 1, S);
+    cfg.blockDim = dim3(TILE_THREADS); cfg.dynamicSmemBytes = TILE_SMEM; cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
-    cfg.attrs = attr; cfg.numAttrs = S > 1 ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, mxfp4_tile_kernel, tmX, tmW, a);
+    attr[0].val.clusterDim.x = PAIR ? 2 : 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
+    cfg.attrs = attr; cfg.numAttrs = PAIR || S > 1 ? 1 : 0;
+    return (int)cudaLaunchKernelEx(&cfg, mxfp4_tile_kernel<PAIR>, tmX, tmW, a);
 }
 // whether TMA can bring the rows of x
 static bool tile_ok(const MxGemm &g) { return g.x_vec && g.ldx >= g.K; }
 
-// The tile's width and the split of K that finish first: rounds of tiles over the SMs times what a tile takes, in SM cycles - a stage the
-// longer of its MMAs (4 BN) and its unpacking, and once a tile its start and epilogue.
-static void tile_plan(int M, int N, int K, int n_sm, int &bn, int &S) {
-    const int tiles_k = mx_tiles(K), tiles_n = mx_tiles(N);
+// The form, the tile's width and the split of K that finish first: rounds of tiles over the SMs times what a tile takes, in SM cycles - a
+// stage the longer of its MMAs (4 BN) and its unpacking, and once a tile its start and epilogue.
+static void tile_plan(int M, int N, int K, int n_sm, bool &pair, int &bn, int &S) {
+    const int tiles_k = mx_tiles(K);
     double best = 1e30;
-    for (int b = 16; b <= 256; b += 16) {
-        if (b > 16 && b - 16 >= M) break;                            // wider than the rows there are
-        const long long tiles = (long long)((M + b - 1) / b) * tiles_n;
-        for (int s = 1; s <= 8; s++) {
-            if (s > 1 && tiles * s > n_sm) break;
-            const int kb = (tiles_k + s - 1) / s;
-            const double stage = 4.0 * b > 450 ? 4.0 * b : 450;
-            const double tile = kb * stage + 1500 + 6.0 * b + (s > 1 ? 1500 + 12.0 * b : 0);
-            const double cost = (double)((tiles * s + n_sm - 1) / n_sm) * tile;
-            if (cost < best) { best = cost; bn = b; S = s; }
+    for (int p = 0; p < 2; p++) {
+        const int rows = p ? 2 * TILE_ROWS : TILE_ROWS, tiles_n = (N + rows - 1) / rows, units = p ? n_sm / 2 : n_sm;
+        for (int b = 16; b <= 256; b += 16) {
+            if (b > 16 && b - 16 >= M) break;                        // wider than the rows there are
+            const long long tiles = (long long)((M + b - 1) / b) * tiles_n;
+            for (int s = 1; s <= (p ? 1 : 8); s++) {
+                if (s > 1 && tiles * s > units) break;
+                const int kb = (tiles_k + s - 1) / s;
+                const double mma = (p ? 4.0 : 5.0) * b, stage = mma > TILE_UNPACK ? mma : TILE_UNPACK;
+                const double tile = kb * stage + 2500 + 4.0 * b + (s > 1 ? 1500 + 12.0 * b : 0);
+                const double cost = (double)((tiles * s + units - 1) / units) * tile;
+                if (cost < best) { best = cost; pair = p; bn = b; S = s; }
+            }
         }
     }
 }
@@ -517,21 +570,31 @@ static int mx_check(const MxGemm &a) {
     return 0;
 }
 
-extern "C" int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
-                             int M, int N, int K, cudaStream_t stream) {
+// form: 0 by the rule; 1 the kernel for few rows, 2 tiles, 3 tiles of pairs of CTAs, with `bn` tokens a tile (a multiple of 16) and K split
+// over `splits` CTAs (form 2): for tests and measurements
+extern "C" int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
+                                 int M, int N, int K, int form, int bn, int splits, cudaStream_t stream) {
     MxGemm a = {(const bf16 *)x, (const uint8_t *)w, (const uint8_t *)scales, out, ldx, ldo, M, N, K, out_dtype, accumulate, 0, nullptr, 0, 0};
     const int bad = mx_check(a);
     if (bad) return bad;
     if (M == 0) return 0;
     a.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
+    if (form == 0) {
+        bool pair = false;
+        form = M > 16 && tile_ok(a) ? 2 : 1;
+        if (form == 2) tile_plan(M, N, K, mx_sm_count(), pair, bn, splits);
+        if (pair) form = 3;
+    } else if (form < 1 || form > 3 || (form > 1 && (!tile_ok(a) || bn < 16 || bn > 256 || bn % 16 || splits < 1 || splits > 8 || (form == 3 && splits > 1))))
+        return FG_ERR_BAD_SIZE;
+    if (form == 2) return launch_tiles<false>(a, bn, splits, stream);
+    if (form == 3) return launch_tiles<true>(a, bn, 1, stream);
     if (M <= 8) return launch_stream<1>(a, 1, stream);
-    if (M > 16 && tile_ok(a)) {
-        int bn, S;
-        tile_plan(M, N, K, mx_sm_count(), bn, S);
-        return launch_tiles(a, bn, S, M, stream);
-    }
     if (M > 65535 * 16) return FG_ERR_BAD_SIZE;
     return launch_stream<2>(a, (M + 15) / 16, stream);
+}
+extern "C" int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
+                             int M, int N, int K, cudaStream_t stream) {
+    return fg_gemm_mxfp4_ext(x, ldx, w, scales, out, out_dtype, ldo, accumulate, M, N, K, 0, 0, 0, stream);
 }
 
 // offsets: [experts + 1] on the device; w, scales: the experts' matrices one after another
@@ -543,7 +606,7 @@ extern "C" int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w
     if (experts <= 0 || experts > 65535 || !offsets) return FG_ERR_BAD_SIZE;
     if (M == 0) return 0;
     a.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
-    if (M > 16ll * experts && experts <= TILE_MAX_EXPERTS && tile_ok(a)) return launch_tiles(a, 128, 1, M, stream);
+    if (M > 16ll * experts && experts <= TILE_MAX_EXPERTS && tile_ok(a)) return launch_tiles<true>(a, 128, 1, stream);
     return (long long)M <= 4ll * experts ? launch_stream<1>(a, experts, stream) : launch_stream<2>(a, experts, stream);
 }
 

@@ -39,11 +39,28 @@ __device__ __forceinline__ void mx_unpack8(uint32_t w, uint32_t (&r)[4]) {
     r[2] = ((h & 0x000f000fu) * 0x1040u) & 0x81c081c0u;
     r[3] = ((h & 0x00f000f0u) * 0x0104u) & 0x81c081c0u;
 }
-// The factor for those numbers: 2^126 2^(e - 127) as a pair of bfloat16, which is a finite power up to e = 128 (a scale of 2;
-// weights' are far below 1).  Larger exponents go by mx_scale_large, in two exact steps.
+// The factor for those numbers: 2^126 2^(e - 127) as a pair of bfloat16, which is a finite power up to e = 128 (a scale of 2; weights' are
+// far below 1).  For larger e it stays at e = 128 and mx_factor_rest is the rest, a second exact step (255: no number).
 __device__ __forceinline__ bool mx_small(uint32_t e) { return e <= 128; }
-__device__ __forceinline__ uint32_t mx_factor(uint32_t e) { return ((e + 126) << 7) * 0x00010001u; }
-__device__ __forceinline__ uint32_t mx_scale_large(uint32_t r, uint32_t e) {
-    const uint32_t p = e == 255 ? 0x7fffu : e == 0 ? 0x0040u : e << 7;
-    return mul_bf16x2(mul_bf16x2(r, 0x7e807e80u), p * 0x00010001u);
+__device__ __forceinline__ uint32_t mx_factor(uint32_t e) { return ((min(e, 128u) + 126) << 7) * 0x00010001u; }
+__device__ __forceinline__ uint32_t mx_factor_rest(uint32_t e) {
+    return (e == 255 ? 0x7fffu : e <= 128 ? 0x3f80u : (e - 1) << 7) * 0x00010001u;
+}
+// A block of 32 numbers with exponent e as bfloat16, in order.  Called by whole warps.
+__device__ __forceinline__ void mx_unpack32(const uint4 &d, uint32_t e, uint32_t (&out)[16]) {
+    const uint32_t w[4] = {d.x, d.y, d.z, d.w}, f = mx_factor(e);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        uint32_t v[4];
+        mx_unpack8(w[u], v);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = mul_bf16x2(v[j], f);
+        out[4 * u] = __byte_perm(v[0], v[1], 0x5410); out[4 * u + 1] = __byte_perm(v[2], v[3], 0x5410);
+        out[4 * u + 2] = __byte_perm(v[0], v[1], 0x7632); out[4 * u + 3] = __byte_perm(v[2], v[3], 0x7632);
+    }
+    if (!__all_sync(0xffffffffu, mx_small(e))) {
+        const uint32_t rest = mx_factor_rest(e);
+#pragma unroll
+        for (int j = 0; j < 16; j++) out[j] = mul_bf16x2(out[j], rest);
+    }
 }

@@ -24,6 +24,8 @@ register_signatures("mx", {
     "fg_mxfp4_quantize": [c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "fg_mxfp4_rows": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_float, c_void_p],
     "fg_gemm_mxfp4": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p],
+    "fg_gemm_mxfp4_ext": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                          c_void_p],
     "fg_gemm_mxfp4_grouped": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int,
                               c_void_p],
     "fg_gemm_mxfp4_error": [],

@@ -255,6 +255,38 @@ def test_contraction(m, n, k):
     plain.check(out, want + res.double().cpu(), slack + 2.0 ** -24 * res.double().cpu().abs())
 
 
+def _named(x, w, form, bn=16, splits=1, dtype=torch.float32):
+    """The contraction by a kernel of the test's choice, into rows with a stride."""
+    m, n = x.shape[0], w.rows
+    room = torch.full((m, n + 2), 7.0, dtype=dtype, device="cuda")
+    out = room[:, 1:n + 1]
+    code = ops.lib("mx").fg_gemm_mxfp4_ext(x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), int(dtype == torch.bfloat16),
+                                           out.stride(0), 0, m, n, w.k, form, bn, splits, torch.cuda.current_stream().cuda_stream)
+    assert code == 0 and (room[:, 0] == 7).all() and (room[:, n + 1:] == 7).all()
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,bn,splits", [(1, 16, 1), (2, 16, 1), (2, 48, 3), (2, 112, 8), (2, 256, 1), (2, 256, 2), (3, 16, 1), (3, 80, 1), (3, 240, 1), (3, 256, 1)])
+@pytest.mark.parametrize("m,n,k", [(1, 100, 32), (70, 129, 96), (40, 513, 1056), (300, 384, 2080), (777, 1000, 160)])
+def test_every_kernel_at_every_width(form, bn, splits, m, n, k):
+    x, (w, numbers) = _rows(m, k, m + n).cuda(), _matrix(n, k, n + k)
+    want, slack = plain.product(x, numbers)
+    plain.check(_named(x, w, form, bn, splits), want, slack)
+    plain.check(_named(x, w, form, bn, splits, torch.bfloat16), want, slack)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,bn", [(2, 32), (3, 32), (3, 256)])
+def test_many_tiles_a_processor(form, bn):
+    """Every SM walks several tiles, of one stage of K and of many."""
+    for m, n, k in ((1500, 1300, 32), (1500, 1300, 128), (900, 5000, 352), (2048, 4096, 1024)):
+        x, (w, numbers) = _rows(m, k, m + n).cuda(), _matrix(n, k, n + k)
+        want = (x.double() @ numbers.cuda().T).cpu()
+        size = (x.double().abs() @ numbers.cuda().abs().T).cpu()
+        plain.check(_named(x, w, form, bn), want, size * (2 * k / 16 + 32) * 2.0 ** -23)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 5, 16, 40, 130, 300])
 def test_contraction_on_strided_rows(m):
