@@ -104,10 +104,7 @@ mxfp4_stream_kernel(MxGemm a) {
                         v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
                     }
                 }
-                // pairs (i, i + 4), as mx_unpack8 gives the weights
-                const uint4 q = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                                           __byte_perm(v.y, v.w, 0x7632));
-                xs[((c * NT + (tok >> 3)) * 4 + (p & 3)) * 32 + (tok & 7) * 4 + (p >> 2)] = q;
+                xs[((c * NT + (tok >> 3)) * 4 + (p & 3)) * 32 + (tok & 7) * 4 + (p >> 2)] = v;
             }
             __syncthreads();
             for (int c = s0 + kg; c < s1; c += STREAM_KG) {
@@ -209,10 +206,10 @@ static int launch_stream(MxGemm a, int y, cudaStream_t stream) {
 //   warp 0      tokens: two boxes of 64 numbers a stage, a ring of up to four
 //   warp 1      MMA issuer: eight 128 x BN x 16 a stage; its commit frees the stage's tokens and its slot of tensor memory (four of 64 columns)
 //   warp 2      weights: 64 bytes a row and 512 bytes of exponents a stage, a ring of six
-//   warps 3-18  four to a lane group of tensor memory, for the halves of the even and of the odd stages: unpack, and at a tile's end its
-//               epilogue.  The first stages of the next tile are unpacked BEFORE a tile's epilogue: the tensor core goes on meanwhile.
-// A stage's unpacking takes a warp about 1,100 cycles from its wait for the weights to its arrival, most of it latency, and a stage's MMAs
-// 1,024 at 256 tokens: two warps a scheduler do not keep up (2,048 x 8,192 x 4,096: 133 us), four do.
+//   warps 3-18  four sets of four, a set to a slot: unpack every fourth stage, and at a tile's end a quarter of its epilogue.  The first
+//               stages of the next tile are unpacked BEFORE a tile's epilogue: the tensor core goes on meanwhile.
+// Unpacking is bound by the integer pipe when enough warps hide the waits around it: with two warps a scheduler, half a stage each, a
+// stage's took 1,500 cycles beside the 1,024 of its MMAs at 256 tokens (2,048 x 8,192 x 4,096: 133 us; with four: 94).
 //
 // One CTA an SM walks the tiles.  PAIR: two CTAs of a cluster take 256 weight rows x BN tokens (tcgen05.mma.cta_group::2); each unpacks its
 // own 128 rows and brings half of the tokens, which halves the bytes an SM receives per MMA.  With few tiles a cluster of single CTAs splits
@@ -296,7 +293,7 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     const int bn = a.bn, xs = a.xs, S = gridDim.z, tiles_k = mx_tiles(a.g.K);
     const int rank = PAIR ? (int)(blockIdx.x & 1) : 0, first = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, stride = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
     const int x_half = (PAIR ? bn / 2 : bn) * 128, x_bytes = 2 * x_half;
-    // full[slot]: a stage's weights are in tensor memory (eight warps a CTA) and its tokens in shared memory; done[slot]: its MMAs are complete
+    // full[slot]: a stage's weights are in tensor memory (four warps a CTA) and its tokens in shared memory; done[slot]: its MMAs are complete
     const uint32_t wfull0 = smem_u32(&bars[0]), wempty0 = wfull0 + 8 * TILE_W_STAGES, full0 = wempty0 + 8 * TILE_W_STAGES, done0 = full0 + 8 * TILE_SLOTS,
                    tfull = done0 + 8 * TILE_SLOTS, tempty = tfull + 8;
     const uint32_t smem0 = smem_u32(smem);
@@ -304,12 +301,13 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     const int kb0 = blockIdx.z * a.kb_per_split, nkb = min(a.kb_per_split, tiles_k - kb0);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < TILE_W_STAGES; s++) { mbar_init(wfull0 + 8 * s, 1); mbar_init(wempty0 + 8 * s, 8); }
-        for (int s = 0; s < TILE_SLOTS; s++) { mbar_init(full0 + 8 * s, PAIR ? 17 : 9); mbar_init(done0 + 8 * s, 1); }
+        for (int s = 0; s < TILE_W_STAGES; s++) { mbar_init(wfull0 + 8 * s, 1); mbar_init(wempty0 + 8 * s, 4); }
+        for (int s = 0; s < TILE_SLOTS; s++) { mbar_init(full0 + 8 * s, PAIR ? 9 : 5); mbar_init(done0 + 8 * s, 1); }
         mbar_init(tfull, 1);
         mbar_init(tempty, PAIR ? 32 : 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (threadIdx.x == 64) { tma_prefetch_map(&tmX); tma_prefetch_map(&tmW); }
     if (warp == 1) { if (PAIR) tc_alloc_pair(smem_u32(&tmem_base_s), 512); else tc_alloc(smem_u32(&tmem_base_s), 512); }
     if (a.g.offsets && warp == 0) {                 // tiles of x in front of each expert's run
         int sum = 0;
@@ -408,38 +406,38 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         for (int j = max(0, issued - TILE_W_STAGES); j < issued; j++) mbar_wait(wfull0 + 8 * (j % TILE_W_STAGES), (j / TILE_W_STAGES) & 1);
     } else {
         // ------------------------------------------------------------ unpack, epilogue
-        const int lg = warp & 3, set = (warp - 3) >> 2, half = set & 1, parity = set >> 1, r = lg * 32 + lane;
+        const int lg = warp & 3, set = (warp - 3) >> 2, r = lg * 32 + lane;
         const uint32_t trow = tmem + ((uint32_t)(lg * 32) << 16);
         const uint32_t full = PAIR ? mapa_u32(full0, 0) : full0, empty = PAIR ? mapa_u32(tempty, 0) : tempty;
-        int g = 0, i = 0;                           // the stage this tile starts with, tiles finished
+        int i = 0;                                  // tiles finished
         bool ok = true;
-        auto unpack = [&](int stage) {
-            const int s = stage % TILE_W_STAGES, slot = stage % TILE_SLOTS;
+        auto unpack = [&](int stage) {              // (stage % TILE_SLOTS == set)
+            const int s = stage % TILE_W_STAGES;
             ok = mbar_wait_warp(wfull0 + 8 * s, (stage / TILE_W_STAGES) & 1);
             if (!ok) { mx_raise(3); return; }
-            const uint8_t *ws = wring + s * TILE_W_STAGE;
-            const uint32_t se = *(const unsigned short *)(ws + TILE_W_BYTES + lane * 16 + lg * 4 + half * 2);
-            uint4 d[2];                             // (64 bytes a row, sixteen-byte pieces swizzled by the row)
+            const uint8_t *ws = wring + s * TILE_W_STAGE, *wr = ws + r * 64;
+            const uint32_t se = *(const uint32_t *)(ws + TILE_W_BYTES + lane * 16 + lg * 4);
+            uint4 d[4];                             // (64 bytes a row, sixteen-byte pieces swizzled by the row)
 #pragma unroll
-            for (int q = 0; q < 2; q++) d[q] = *(const uint4 *)(ws + r * 64 + (((half * 2 + q) ^ ((r >> 1) & 3)) << 4));
-            __syncwarp();
-            if (lane == 0) mbar_arrive(wempty0 + 8 * s);
+            for (int q = 0; q < 4; q++) d[q] = *(const uint4 *)(wr + ((q ^ ((r >> 1) & 3)) << 4));
             if (stage >= TILE_SLOTS) {
-                ok = mbar_wait_warp(done0 + 8 * slot, (stage / TILE_SLOTS - 1) & 1);
+                ok = mbar_wait_warp(done0 + 8 * set, (stage / TILE_SLOTS - 1) & 1);
                 if (!ok) { mx_raise(7); return; }
             }
             tc_fence_after();
-            const uint32_t at = trow + 256 + slot * 64 + half * 32;
 #pragma unroll
-            for (int q = 0; q < 2; q++) {           // a block of 32 numbers
+            for (int q = 0; q < 4; q++) {           // a block of 32 numbers
                 uint32_t out[16];
                 mx_unpack32(d[q], (se >> (8 * q)) & 255, out);
-                tc_st16(at + q * 16, out);
+                tc_st16(trow + 256 + set * 64 + q * 16, out);
             }
             tc_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) { if (PAIR) mbar_arrive_cluster(full + 8 * slot); else mbar_arrive(full + 8 * slot); }
+            if (lane == 0) {
+                if (PAIR) mbar_arrive_cluster(full + 8 * set); else mbar_arrive(full + 8 * set);
+                mbar_arrive(wempty0 + 8 * s);
+            }
         };
         auto epilogue = [&](int T) {
             const MxTile t = mx_tile<PAIR>(a, cum, T, rank);
@@ -469,15 +467,19 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
             for (int q = 0; q < 4; q++)
                 if ((4 * q + set) * 16 < bn) tile_store(a.g, t.m0 + (4 * q + set) * 16, t.m_end, n, v[q]);
         };
-        // (one loop, so that the code of each stands once: the epilogue of the tile `before` comes behind the first stages of the next)
-        for (int T = first, before = -1; ; before = T, T += stride) {
-            const int stages = T < n_tiles && ok ? nkb : 0, lead = min(stages, TILE_AHEAD);
-            for (int kb = 0; kb <= stages; kb++) {
-                if (kb == lead && before >= 0) { epilogue(before); i++; }
-                if (kb < stages && ok && ((g + kb) & 1) == parity) unpack(g + kb);
-            }
-            if (stages == 0) break;
-            g += stages;
+        // A tight loop over this set's stages up to `limit`, what happens between tiles outside of it: the epilogue of the tile `before` comes
+        // behind the first stages of the next one.
+        int T = first, before = -1, st = set;
+        bool more = T < n_tiles;
+        int g_end = more ? nkb : 0, limit = g_end;
+        while (more || before >= 0) {
+            for (; st < limit && ok; st += TILE_SLOTS) unpack(st);
+            if (before >= 0) { epilogue(before); i++; before = -1; }
+            if (!more) break;
+            if (limit < g_end && ok) { limit = g_end; continue; }
+            before = T; T += stride;
+            more = T < n_tiles && ok;
+            if (more) { limit = g_end + min(nkb, TILE_AHEAD); g_end += nkb; }
         }
         tc_fence_before();
     }

@@ -28,16 +28,24 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-// Eight numbers (a 32-bit word) as bfloat16 times 2^-126: r[j] holds number j in its low and number j + 4 in its high half.
+// bytes of a and b by four selectors of four bits; bit 3 of one asks for eight copies of its byte's top bit
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "n"(SEL));
+    return d;
+}
+// Eight numbers (a 32-bit word) as bfloat16 times 2^-126, in order, two to a word.
 // The three bits below a code's sign, put at the bottom of a bfloat16's exponent field and the top of its mantissa, are the
-// number times 2^-126 (1/2 as a subnormal).  One multiplication by 2^12 + 2^6 puts sign and value in place for two numbers:
-// the copies (bits 12..15 and 6..9 of each half) do not overlap, so nothing carries.
+// number times 2^-126 (1/2 as a subnormal).  The even and the odd codes are masked to a byte each; a byte permutation puts the two of a
+// word into its halves, with zeros beside them (the sign of a byte below 128, replicated); one multiplication by 2^12 + 2^6 moves sign and
+// value of both into place: the copies (bits 12..15 and 6..9 of each half) do not overlap, so nothing carries.
 __device__ __forceinline__ void mx_unpack8(uint32_t w, uint32_t (&r)[4]) {
-    const uint32_t h = w >> 8;
-    r[0] = ((w & 0x000f000fu) * 0x1040u) & 0x81c081c0u;
-    r[1] = ((w & 0x00f000f0u) * 0x0104u) & 0x81c081c0u;
-    r[2] = ((h & 0x000f000fu) * 0x1040u) & 0x81c081c0u;
-    r[3] = ((h & 0x00f000f0u) * 0x0104u) & 0x81c081c0u;
+    const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+    r[0] = (prmt<0xc480u>(even, odd) * 0x1040u) & 0x81c081c0u;
+    r[1] = (prmt<0xd591u>(even, odd) * 0x1040u) & 0x81c081c0u;
+    r[2] = (prmt<0xe6a2u>(even, odd) * 0x1040u) & 0x81c081c0u;
+    r[3] = (prmt<0xf7b3u>(even, odd) * 0x1040u) & 0x81c081c0u;
 }
 // The factor for those numbers: 2^126 2^(e - 127) as a pair of bfloat16, which is a finite power up to e = 128 (a scale of 2; weights' are
 // far below 1).  For larger e it stays at e = 128 and mx_factor_rest is the rest, a second exact step (255: no number).
@@ -54,9 +62,7 @@ __device__ __forceinline__ void mx_unpack32(const uint4 &d, uint32_t e, uint32_t
         uint32_t v[4];
         mx_unpack8(w[u], v);
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = mul_bf16x2(v[j], f);
-        out[4 * u] = __byte_perm(v[0], v[1], 0x5410); out[4 * u + 1] = __byte_perm(v[2], v[3], 0x5410);
-        out[4 * u + 2] = __byte_perm(v[0], v[1], 0x7632); out[4 * u + 3] = __byte_perm(v[2], v[3], 0x7632);
+        for (int j = 0; j < 4; j++) out[4 * u + j] = mul_bf16x2(v[j], f);
     }
     if (!__all_sync(0xffffffffu, mx_small(e))) {
         const uint32_t rest = mx_factor_rest(e);
