@@ -32,28 +32,49 @@ __device__ __forceinline__ void mx_store(const MxGemm &a, int m, int n, float v)
     else ((bf16 *)a.out)[at] = __float2bfloat16_rn(v);
 }
 
-// ---------------------------------------------------------------------------- few rows: weights straight from memory to the MMA
-// A CTA takes 64 weight rows and a share of K, its eight warps two sets of 32 rows x four interleaved shares of the chunks of 128 numbers.
-// Weight rows are the M side of mma.sync.m16n8k16, tokens its N side.  The order of k inside a chunk is free as long as both operands
-// follow it: lane (g, t) of a warp reads 16 bytes - block t of the chunk, 32 numbers that share one exponent - of row g of each of
-// four groups of eight rows, and feeds them to the eight MMAs of the chunk as they come, so that weights go from global memory to the
-// tensor core through registers alone.  x lies in shared memory in that order.  The four shares of K are added in shared memory, the CTAs
-// of a cluster (a split of K where there are few weight rows) through distributed shared memory, both in a fixed order.
-#define STREAM_ROWS 64
-#define STREAM_KG 4
-#define STREAM_CHUNKS(NT) (32 / (NT))       // chunks of x that are staged at once: 64 KB
+// ---------------------------------------------------------------------------- few rows: weights through a warp's own ring to the MMA
+// Weight rows are the M side of mma.sync.m16n8k16, tokens its N side.  A warp takes 32 weight rows x chunks of 128 numbers of K; lane (g, t)
+// of it handles 16 bytes - block t of the chunk, 32 numbers that share one exponent - of row g of each of four groups of eight rows and
+// feeds them to the eight MMAs of the chunk as they come: the order of k inside a chunk is free as long as both operands follow it.  x lies
+// in shared memory in the lanes' order.  Every lane copies what it will use itself, asynchronously and three chunks ahead (104 KB in flight
+// on an SM, with no registers held for them), so the ring needs no barrier.
+//
+// What bounds it: instructions.  At the memory's rate an SM gets a chunk's 2,176 bytes of 32 rows every 92 cycles, in which its four
+// schedulers issue 368; unpacking them takes 192, the MMAs, loads and addresses some 70.
+//
+// A CTA is two groups of eight warps; a group takes a unit of 32 rows at a time, its warps a chunk each in turn.  x is staged once for all the
+// units of a CTA (in parts, for each unit again, where K is longer than the room).  The eight sums are added in shared memory, those of a cluster's
+// CTAs (a split of K where there are few units, or K is long) through distributed shared memory, all in a fixed order.
+#define STREAM_ROWS 32
+#define STREAM_WARPS 8                      // of a group
+#define STREAM_GROUPS 2
+#define STREAM_THREADS (32 * STREAM_WARPS * STREAM_GROUPS)
+#define STREAM_RING(NT) ((NT) == 1 ? 4 : 3)  // chunks in a warp's ring (at 16 tokens the partial sums take the room of one)
+#define STREAM_SLOT 2176                    // 32 rows x 64 bytes, and 128 bytes of exponents
+#define STREAM_CHUNKS(NT) (32 / (NT))       // chunks of x staged at once: 64 KB
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 
 template <int NT>
-__global__ void __launch_bounds__(256, 2)
-mxfp4_stream_kernel(MxGemm a) {
+__global__ void __launch_bounds__(STREAM_THREADS, 1)
+mxfp4_stream_kernel(const MxGemm a, int units) {
     extern __shared__ __align__(16) uint8_t smem[];
-    uint4 *xs = (uint4 *)smem;                                        // [chunk][NT][4][32 lanes] of 8 bfloat16
-    float *red = (float *)smem;                                       // [KG][8 NT tokens][64 rows], once x is no longer needed
+    // [warp][RING] slots of weights | [group][warp][8 NT tokens][32 rows] partial sums | x: [chunk][NT][4][32 lanes] of 8 numbers
+    constexpr int RING = STREAM_RING(NT), RED = STREAM_WARPS * 8 * NT * STREAM_ROWS;
+    float *red_all = (float *)(smem + STREAM_GROUPS * STREAM_WARPS * RING * STREAM_SLOT);
+    uint4 *xs = (uint4 *)(red_all + STREAM_GROUPS * RED);
     const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rg = warp & 1, kg = warp >> 1;
-    const int tile = blockIdx.x, S = gridDim.z;
-    const int tiles_k = mx_tiles(a.K), blocks = a.K / MX_BLOCK;
+    const int group = warp / STREAM_WARPS, wl = warp % STREAM_WARPS, tid = threadIdx.x & (32 * STREAM_WARPS - 1);
+    float *red = red_all + group * RED;
+    const uint32_t ring = smem_u32(smem) + warp * RING * STREAM_SLOT;
+    const int S = gridDim.z, tiles_k = mx_tiles(a.K), blocks = a.K / MX_BLOCK;
     const int c_begin = blockIdx.z * a.chunks_per_split, c_end = min(tiles_k, c_begin + a.chunks_per_split);
+    const bool in_parts = c_end - c_begin > STREAM_CHUNKS(NT);
     const uint8_t *w = a.w, *sc = a.sc;
     int m_begin, m_end;
     if (a.offsets) {
@@ -62,139 +83,179 @@ mxfp4_stream_kernel(MxGemm a) {
         w += (size_t)e * a.N * (a.K / 2);
         sc += (size_t)e * mx_scale_bytes(a.N, a.K);
     } else { m_begin = blockIdx.y * 8 * NT; m_end = min(a.M, m_begin + 8 * NT); }
-    // this warp's rows: eight neighbouring rows (i8 ..) of each quarter of a tile of 128, whose exponents are 128 neighbouring bytes
-    const int base = (tile >> 1) * 128, i8 = ((tile & 1) * 2 + rg) * 8;
-    const uint8_t *wrow[4];
-    bool row_ok[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int r = base + 32 * j + i8 + g;
-        row_ok[j] = r < a.N;
-        wrow[j] = w + (size_t)(row_ok[j] ? r : 0) * (a.K / 2) + t * 16;
-    }
-    const uint8_t *srow = sc + (size_t)(tile >> 1) * tiles_k * MX_TILE_BYTES + (i8 + g) * 16;
+    const size_t pitch = a.K / 2;
+    const int first = blockIdx.x * STREAM_GROUPS + group, stride = gridDim.x * STREAM_GROUPS;
+    auto group_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * STREAM_WARPS) : "memory"); };
 
     for (int m0 = m_begin; m0 < m_end; m0 += 8 * NT) {
-        float acc[2][NT][4];
+        // What is copied next: chunk fc of unit fu.  Unit u is eight neighbouring rows (from 8 (u % 4)) of each quarter of a tile of 128, whose
+        // exponents are 128 neighbouring bytes.  Rows past the last read that one (their sums are not stored), blocks past the end of K the row's
+        // first (x is zero there).
+        int fu = first - stride, fc = c_end, fs = 0;
+        const uint8_t *row[4], *exps = nullptr;
+        auto copy = [&] {
+            if (fc >= c_end) {
+                fu += stride;
+                fc = c_begin + wl;
+                if (fu < units) {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+                    for (int j = 0; j < 4; j++) row[j] = w + min((fu >> 2) * 128 + 32 * j + (fu & 3) * 8 + g, a.N - 1) * pitch + t * 16;
+                    exps = sc + (size_t)(fu >> 2) * tiles_k * MX_TILE_BYTES + ((fu & 3) * 8 + g) * 16;
+                }
+            }
+            if (fu < units && fc < c_end) {
+                const int at = fc * 4 + t < blocks ? fc * 64 : -t * 16;
+                const uint32_t dst = ring + fs * STREAM_SLOT + lane * 16;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+                for (int j = 0; j < 4; j++) cp_async16(dst + j * 512, row[j] + at);
+                if (t == 0) cp_async16(ring + fs * STREAM_SLOT + 2048 + g * 16, exps + fc * MX_TILE_BYTES);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            fc += STREAM_WARPS;
+            fs = fs + 1 == RING ? 0 : fs + 1;
+        };
+        for (int i = 0; i < RING - 1; i++) copy();
+        int s = 0;                                                    // the slot that is used next
+        bool staged = false;
+        // (both groups walk as many rounds: the barriers of the whole CTA are met by all)
+        for (int u0 = blockIdx.x * STREAM_GROUPS; u0 < units; u0 += stride) {
+            const int u = u0 + group;
+            const bool live = u < units;
+            float sum[2][NT][4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][n][j] = 0.f;
-        for (int s0 = c_begin; s0 < c_end; s0 += STREAM_CHUNKS(NT)) {
-            const int s1 = min(c_end, s0 + STREAM_CHUNKS(NT));
-            uint4 d[4], e4;
-            auto fetch = [&](int c) {
-                const bool live = c < s1 && c * 4 + t < blocks;
+            for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) d[j] = live && row_ok[j] ? __ldcs((const uint4 *)(wrow[j] + (size_t)c * 64)) : make_uint4(0, 0, 0, 0);
-                e4 = c < s1 ? *(const uint4 *)(srow + (size_t)c * MX_TILE_BYTES) : make_uint4(0, 0, 0, 0);
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sum[i][n][j] = 0.f;
+            for (int s0 = c_begin; s0 < c_end; s0 += STREAM_CHUNKS(NT)) {
+                const int s1 = min(c_end, s0 + STREAM_CHUNKS(NT));
+                if (!staged || in_parts) {
+                    __syncthreads();                                  // the last use of x is over
+                    const int pieces = (s1 - s0) * NT * 128;          // of eight numbers: [chunk][token][16]
+#pragma unroll 4
+                    for (int q = threadIdx.x; q < pieces; q += STREAM_THREADS) {
+                        const int p = q & 15, tok = (q >> 4) & (8 * NT - 1), c = (q >> 7) / NT, k = (s0 + c) * 128 + p * 8;
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (m0 + tok < m_end && k < a.K) {
+                            const bf16 *src = a.x + (size_t)(m0 + tok) * a.ldx + k;
+                            if (a.x_vec) v = *(const uint4 *)src;
+                            else {
+                                const unsigned short *h = (const unsigned short *)src;
+                                v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                            }
+                        }
+                        xs[((c * NT + (tok >> 3)) * 4 + (p & 3)) * 32 + (tok & 7) * 4 + (p >> 2)] = v;
+                    }
+                    __syncthreads();
+                    staged = true;
+                }
+                if (!live) continue;
+                for (int c = s0 + wl; c < s1; c += STREAM_WARPS) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
+                    __syncwarp();                                     // the exponents were copied by other lanes
+                    const uint32_t slot = ring + s * STREAM_SLOT;
+                    const uint4 ee = lds128(slot + 2048 + g * 16);
+                    uint4 d[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) d[j] = lds128(slot + j * 512 + lane * 16);
+                    const uint32_t e[4] = {(ee.x >> (8 * t)) & 255, (ee.y >> (8 * t)) & 255, (ee.z >> (8 * t)) & 255, (ee.w >> (8 * t)) & 255};
+                    __syncwarp();
+                    copy();                                           // into the slot that was used last
+                    const uint4 *xc = xs + (c - s0) * NT * 128 + lane;
+                    const bool small = __all_sync(0xffffffffu, mx_small(max(max(e[0], e[1]), max(e[2], e[3]))));
+                    uint32_t f[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) f[j] = mx_factor(e[j]);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t v[4][4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            mx_unpack8(q == 0 ? d[j].x : q == 1 ? d[j].y : q == 2 ? d[j].z : d[j].w, v[j]);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) v[j][i] = mul_bf16x2(v[j][i], f[j]);
+                        }
+                        if (!small)
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++) v[j][i] = mx_times_rest(v[j][i], e[j]);
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            const uint4 b = xc[(n * 4 + q) * 32];
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                mma_bf16_16x8x16(sum[i][n], v[2 * i][0], v[2 * i + 1][0], v[2 * i][1], v[2 * i + 1][1], b.x, b.y);
+                                mma_bf16_16x8x16(sum[i][n], v[2 * i][2], v[2 * i + 1][2], v[2 * i][3], v[2 * i + 1][3], b.z, b.w);
+                            }
+                        }
+                    }
+                    s = s + 1 == RING ? 0 : s + 1;
+                }
+            }
+            // ---- sums of the eight warps, then of the cluster's CTAs
+            const int total = live ? min(8 * NT, m_end - m0) * STREAM_ROWS : 0;
+            auto store = [&](int q, float v) {
+                const int rl = q % STREAM_ROWS, n = (u >> 2) * 128 + (rl >> 3) * 32 + (u & 3) * 8 + (rl & 7);
+                if (n < a.N) mx_store(a, m0 + q / STREAM_ROWS, n, v);
             };
-            fetch(s0 + kg);
-            __syncthreads();                                          // the last use of the shared memory is over
-            for (int u = threadIdx.x; u < (s1 - s0) * NT * 8 * 16; u += 256) {
-                const int p = u & 15, tok = (u >> 4) % (8 * NT), c = (u >> 4) / (8 * NT), k = (s0 + c) * 128 + p * 8;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (m0 + tok < m_end && k < a.K) {
-                    const bf16 *src = a.x + (size_t)(m0 + tok) * a.ldx + k;
-                    if (a.x_vec) v = *(const uint4 *)src;
-                    else {
-                        const unsigned short *h = (const unsigned short *)src;
-                        v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-                    }
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            red[(wl * 8 * NT + n * 8 + 2 * t + (j & 1)) * STREAM_ROWS + (2 * i + (j >> 1)) * 8 + g] = sum[i][n][j];
+                group_sync();
+                for (int q = tid; q < total; q += 32 * STREAM_WARPS) {
+                    float v = red[q];
+#pragma unroll
+                    for (int z = 1; z < STREAM_WARPS; z++) v += red[z * 8 * NT * STREAM_ROWS + q];
+                    if (S == 1) store(q, v); else red[q] = v;
                 }
-                xs[((c * NT + (tok >> 3)) * 4 + (p & 3)) * 32 + (tok & 7) * 4 + (p >> 2)] = v;
+                group_sync();                                         // before the next unit's sums
             }
-            __syncthreads();
-            for (int c = s0 + kg; c < s1; c += STREAM_KG) {
-                const uint4 cur[4] = {d[0], d[1], d[2], d[3]};
-                const uint32_t se[4] = {(e4.x >> (8 * t)) & 255, (e4.y >> (8 * t)) & 255, (e4.z >> (8 * t)) & 255, (e4.w >> (8 * t)) & 255};
-                fetch(c + STREAM_KG);
-                const bool small = __all_sync(0xffffffffu, mx_small(se[0]) && mx_small(se[1]) && mx_small(se[2]) && mx_small(se[3]));
-                const uint4 *xc = xs + (size_t)(c - s0) * NT * 128 + lane;
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    uint32_t r[4][4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        mx_unpack8(u == 0 ? cur[j].x : u == 1 ? cur[j].y : u == 2 ? cur[j].z : cur[j].w, r[j]);
-                        const uint32_t f = mx_factor(se[j]);
-#pragma unroll
-                        for (int q = 0; q < 4; q++) r[j][q] = mul_bf16x2(r[j][q], f);
-                        if (!small) {
-                            const uint32_t rest = mx_factor_rest(se[j]);
-#pragma unroll
-                            for (int q = 0; q < 4; q++) r[j][q] = mul_bf16x2(r[j][q], rest);
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        const uint4 b = xc[(n * 4 + u) * 32];
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            mma_bf16_16x8x16(acc[i][n], r[2 * i][0], r[2 * i + 1][0], r[2 * i][1], r[2 * i + 1][1], b.x, b.y);
-                            mma_bf16_16x8x16(acc[i][n], r[2 * i][2], r[2 * i + 1][2], r[2 * i][3], r[2 * i + 1][3], b.z, b.w);
-                        }
-                    }
+            if (S > 1) {
+                cluster_sync_all();
+                const uint32_t red0 = smem_u32(red);
+                for (int q = blockIdx.z * 32 * STREAM_WARPS + tid; q < total; q += 32 * STREAM_WARPS * S) {
+                    float v = 0.f;
+                    for (int z = 0; z < S; z++) v += ld_dsmem_f32(red0 + q * 4, z);
+                    store(q, v);
                 }
+                cluster_sync_all();                                   // nobody overwrites or leaves what others still read
             }
         }
-        // sums of the four shares of K, then of the cluster's CTAs
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    red[(kg * 8 * NT + n * 8 + 2 * t + (j & 1)) * STREAM_ROWS + rg * 32 + (2 * i + (j >> 1)) * 8 + g] = acc[i][n][j];
-        __syncthreads();
-        const int tokens = min(8 * NT, m_end - m0), total = tokens * STREAM_ROWS;
-        for (int u = threadIdx.x; u < total; u += 256) {
-            float v = red[u];
-#pragma unroll
-            for (int q = 1; q < STREAM_KG; q++) v += red[q * 8 * NT * STREAM_ROWS + u];
-            if (S == 1) {
-                const int rl = u & 63, n = base + ((rl >> 3) & 3) * 32 + ((tile & 1) * 2 + (rl >> 5)) * 8 + (rl & 7);
-                if (n < a.N) mx_store(a, m0 + u / STREAM_ROWS, n, v);
-            } else red[u] = v;
-        }
-        if (S > 1) {
-            cluster_sync_all();
-            const uint32_t red0 = (uint32_t)__cvta_generic_to_shared(red);
-            for (int u = blockIdx.z * 256 + threadIdx.x; u < total; u += 256 * S) {
-                float v = 0.f;
-                for (int z = 0; z < S; z++) v += ld_dsmem_f32(red0 + u * 4, z);
-                const int rl = u & 63, n = base + ((rl >> 3) & 3) * 32 + ((tile & 1) * 2 + (rl >> 5)) * 8 + (rl & 7);
-                if (n < a.N) mx_store(a, m0 + u / STREAM_ROWS, n, v);
-            }
-            cluster_sync_all();                                       // nobody overwrites or leaves what others still read
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
 }
 
 template <int NT>
-static int launch_stream(MxGemm a, int y, cudaStream_t stream) {
-    const int tiles_k = mx_tiles(a.K), tiles_n = 2 * mx_tiles(a.N);      // a tile: eight rows twice in each quarter of 128
+static int launch_stream(MxGemm a, int y, int busy /* of the y, that have rows */, cudaStream_t stream) {
+    const int tiles_k = mx_tiles(a.K), units = 4 * mx_tiles(a.N), room = mx_sm_count();
+    // K over a cluster: until x fits at once, and while there are too few units for the SMs and each warp keeps a chunk
     int S = 1;
-    while (S < 8 && (long long)tiles_n * y * S < 296 && tiles_k > S * STREAM_KG) S *= 2;
+    while (S < 8 && (tiles_k > S * STREAM_CHUNKS(NT) || ((long long)units * busy * S <= room * STREAM_GROUPS / 2 && tiles_k > S * STREAM_WARPS))) S *= 2;
     a.chunks_per_split = (tiles_k + S - 1) / S;
     const int staged = a.chunks_per_split < STREAM_CHUNKS(NT) ? a.chunks_per_split : STREAM_CHUNKS(NT);
-    const int red = STREAM_KG * 8 * NT * STREAM_ROWS * 4, xb = staged * NT * 2048;
-    const int smem = xb > red ? xb : red;
+    constexpr int fixed = STREAM_GROUPS * STREAM_WARPS * (STREAM_RING(NT) * STREAM_SLOT + 8 * NT * STREAM_ROWS * 4);
     static FgPerDevice configured;
     if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(mxfp4_stream_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_CHUNKS(NT) * NT * 2048);
+        cudaError_t e = cudaFuncSetAttribute(mxfp4_stream_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + 65536);
         if (e != cudaSuccess) return (int)e;
     }
+    const int pairs = (units + STREAM_GROUPS - 1) / STREAM_GROUPS;
+    int gx = room / (busy * S);                                      // as many CTAs as fit at once
+    gx = gx < 1 ? 1 : gx > pairs ? pairs : gx;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles_n, y, S); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cfg.gridDim = dim3(gx, y, S); cfg.blockDim = dim3(STREAM_THREADS); cfg.dynamicSmemBytes = fixed + staged * NT * 2048; cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
     cfg.attrs = attr; cfg.numAttrs = S > 1 ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, mxfp4_stream_kernel<NT>, a);
+    return (int)cudaLaunchKernelEx(&cfg, mxfp4_stream_kernel<NT>, a, units);
 }
 
 // ---------------------------------------------------------------------------- more rows: weights through tensor memory
@@ -590,9 +651,9 @@ extern "C" int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, co
         return FG_ERR_BAD_SIZE;
     if (form == 2) return launch_tiles<false>(a, bn, splits, stream);
     if (form == 3) return launch_tiles<true>(a, bn, 1, stream);
-    if (M <= 8) return launch_stream<1>(a, 1, stream);
+    if (M <= 8) return launch_stream<1>(a, 1, 1, stream);
     if (M > 65535 * 16) return FG_ERR_BAD_SIZE;
-    return launch_stream<2>(a, (M + 15) / 16, stream);
+    return launch_stream<2>(a, (M + 15) / 16, (M + 15) / 16, stream);
 }
 extern "C" int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
                              int M, int N, int K, cudaStream_t stream) {
@@ -609,7 +670,7 @@ extern "C" int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w
     if (M == 0) return 0;
     a.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     if (M > 16ll * experts && experts <= TILE_MAX_EXPERTS && tile_ok(a)) return launch_tiles<true>(a, 128, 1, stream);
-    return (long long)M <= 4ll * experts ? launch_stream<1>(a, experts, stream) : launch_stream<2>(a, experts, stream);
+    return (long long)M <= 4ll * experts ? launch_stream<1>(a, experts, M < experts ? M : experts, stream) : launch_stream<2>(a, experts, M < experts ? M : experts, stream);
 }
 
 // 0, or (code << 8 | role) of the first bounded wait that ran out since it was asked last

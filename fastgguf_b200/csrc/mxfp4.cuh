@@ -28,31 +28,25 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-// bytes of a and b by four selectors of four bits; bit 3 of one asks for eight copies of its byte's top bit
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "n"(SEL));
-    return d;
-}
-// Eight numbers (a 32-bit word) as bfloat16 times 2^-126, in order, two to a word.
-// The three bits below a code's sign, put at the bottom of a bfloat16's exponent field and the top of its mantissa, are the
-// number times 2^-126 (1/2 as a subnormal).  The even and the odd codes are masked to a byte each; a byte permutation puts the two of a
-// word into its halves, with zeros beside them (the sign of a byte below 128, replicated); one multiplication by 2^12 + 2^6 moves sign and
-// value of both into place: the copies (bits 12..15 and 6..9 of each half) do not overlap, so nothing carries.
+// Eight numbers (a 32-bit word) as bfloat16 times 2^-129, in order, two to a word.
+// One instruction turns a byte into two half-precision numbers.  Those times 2^-20 are subnormal in half precision, exactly: 16 |q| <= 96
+// units of 2^-24, a sign and an integer in the low seven bits - which are a bfloat16's mantissa, so the SAME bits are the subnormal bfloat16
+// number 16 |q| 2^-133.  A word takes 15 cycles of a scheduler this way, factor included, of which bit operations on the codes take 19 to 23.
 __device__ __forceinline__ void mx_unpack8(uint32_t w, uint32_t (&r)[4]) {
-    const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
-    r[0] = (prmt<0xc480u>(even, odd) * 0x1040u) & 0x81c081c0u;
-    r[1] = (prmt<0xd591u>(even, odd) * 0x1040u) & 0x81c081c0u;
-    r[2] = (prmt<0xe6a2u>(even, odd) * 0x1040u) & 0x81c081c0u;
-    r[3] = (prmt<0xf7b3u>(even, odd) * 0x1040u) & 0x81c081c0u;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\tcvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
+#pragma unroll
+    for (int j = 0; j < 4; j++) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(r[j]) : "r"(0x00100010u));      // 2^-20
 }
-// The factor for those numbers: 2^126 2^(e - 127) as a pair of bfloat16, which is a finite power up to e = 128 (a scale of 2; weights' are
-// far below 1).  For larger e it stays at e = 128 and mx_factor_rest is the rest, a second exact step (255: no number).
-__device__ __forceinline__ bool mx_small(uint32_t e) { return e <= 128; }
-__device__ __forceinline__ uint32_t mx_factor(uint32_t e) { return ((min(e, 128u) + 126) << 7) * 0x00010001u; }
-__device__ __forceinline__ uint32_t mx_factor_rest(uint32_t e) {
-    return (e == 255 ? 0x7fffu : e <= 128 ? 0x3f80u : (e - 1) << 7) * 0x00010001u;
+// The factor for those numbers: 2^129 2^(e - 127) as a pair of bfloat16, a finite power up to e = 125 (a scale of 1/4; weights' are far below).
+// For larger e it stays there and the rest follows in two more exact steps (255: no number).
+__device__ __forceinline__ bool mx_small(uint32_t e) { return e <= 125; }
+__device__ __forceinline__ uint32_t mx_factor(uint32_t e) { return (min(e, 125u) + 129) * 0x00800080u; }
+__device__ __forceinline__ uint32_t mx_times_rest(uint32_t r, uint32_t e) {
+    const uint32_t over = max(e, 125u) - 125, half = over >> 1;
+    r = mul_bf16x2(mul_bf16x2(r, (half + 127) * 0x00800080u), (over - half + 127) * 0x00800080u);
+    return e == 255 ? 0x7fff7fffu : r;
 }
 // A block of 32 numbers with exponent e as bfloat16, in order.  Called by whole warps.
 __device__ __forceinline__ void mx_unpack32(const uint4 &d, uint32_t e, uint32_t (&out)[16]) {
@@ -65,8 +59,7 @@ __device__ __forceinline__ void mx_unpack32(const uint4 &d, uint32_t e, uint32_t
         for (int j = 0; j < 4; j++) out[4 * u + j] = mul_bf16x2(v[j], f);
     }
     if (!__all_sync(0xffffffffu, mx_small(e))) {
-        const uint32_t rest = mx_factor_rest(e);
 #pragma unroll
-        for (int j = 0; j < 16; j++) out[j] = mul_bf16x2(out[j], rest);
+        for (int j = 0; j < 16; j++) out[j] = mx_times_rest(out[j], e);
     }
 }

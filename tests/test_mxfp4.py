@@ -375,6 +375,29 @@ def test_contraction_of_two_quantised_operands(m, n, k):
     assert (room[:, 0] == 7).all() and (room[:, n + 1:] == 7).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(3, 70, 352), (8, 64, 4096), (13, 128, 8192), (16, 40, 32768), (5, 33, 65536)])
+def test_activations_of_any_range(m, n, k):
+    """Few rows: numbers of one token that are many binades apart (the smallest beside the largest, where half precision cannot hold both),
+    tokens of very different sizes, rows of zeros, K longer than what is staged at once."""
+    g = _gen(m + k)
+    x = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-60, 30, (m, 1), generator=g).float())
+    x[0] = 0
+    x[1, ::7] = 0
+    x[2, 5] = 2.0 ** 90                                      # under a weight of 0: nothing of it reaches the sums
+    x[2, 40:] *= 2.0 ** -50
+    x[m - 1] *= torch.exp2(torch.randint(-50, 10, (k,), generator=g).float())
+    x = x.bfloat16()
+    data, e = plain.random_matrix(n, k, g, 117, 123)
+    data[:, 2] &= 15                                         # (number 5: the high half of byte 2)
+    e[3], data[3] = 0, 0                                     # a row of zeros, as the quantiser makes it
+    w, numbers = Mxfp4.from_exponents(data.cuda(), e.cuda()), plain.numbers(data, e)
+    want, slack = plain.product(x, numbers)
+    got = _named(x.cuda(), w, 1)
+    plain.check(got, want, slack)
+    assert (got[0] == 0).all() and (got[:, 3] == 0).all()
+
+
 def _runs(counts, before=0):
     return torch.tensor([before + sum(counts[:i]) for i in range(len(counts) + 1)], dtype=torch.int32)
 
