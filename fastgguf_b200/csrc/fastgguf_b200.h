@@ -409,6 +409,12 @@ int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, const void *s
 /* rows offsets[e] <= m < offsets[e + 1] (device) with matrix e of a stack; rows of no run are not written */
 int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w, const void *scales, const int *offsets, int experts, void *out,
                           int out_dtype, long long ldo, int accumulate, int M, int N, int K, cudaStream_t stream);
+/* the same with x in the format too; ext: bn tokens a tile and `splits` CTAs that share K (0: by the rule) */
+int fg_gemm_mxfp4_both(const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int out_dtype, long long ldo,
+                       int accumulate, int M, int N, int K, cudaStream_t stream);
+int fg_gemm_mxfp4_both_ext(const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int out_dtype, long long ldo,
+                           int accumulate, int M, int N, int K, int bn, int splits, cudaStream_t stream);
+/* 0, or (code << 8 | role) of the first bounded wait of these kernels that ran out since it was asked last */
 int fg_gemm_mxfp4_error(void);
 
 #ifdef __cplusplus

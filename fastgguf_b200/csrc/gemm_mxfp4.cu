@@ -60,6 +60,12 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ uint32_t lds8(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 template <int NT>
 __global__ void __launch_bounds__(STREAM_THREADS, 1)
 mxfp4_stream_kernel(const MxGemm a, int units) {
@@ -155,32 +161,28 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
                     asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
                     __syncwarp();                                     // the exponents were copied by other lanes
                     const uint32_t slot = ring + s * STREAM_SLOT;
-                    const uint4 ee = lds128(slot + 2048 + g * 16);
+                    uint32_t e[4];
                     uint4 d[4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) d[j] = lds128(slot + j * 512 + lane * 16);
-                    const uint32_t e[4] = {(ee.x >> (8 * t)) & 255, (ee.y >> (8 * t)) & 255, (ee.z >> (8 * t)) & 255, (ee.w >> (8 * t)) & 255};
+                    for (int j = 0; j < 4; j++) {
+                        e[j] = lds8(slot + 2048 + g * 16 + t + 4 * j);
+                        d[j] = lds128(slot + j * 512 + lane * 16);
+                    }
                     __syncwarp();
                     copy();                                           // into the slot that was used last
                     const uint4 *xc = xs + (c - s0) * NT * 128 + lane;
-                    const bool small = __all_sync(0xffffffffu, mx_small(max(max(e[0], e[1]), max(e[2], e[3]))));
-                    uint32_t f[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) f[j] = mx_factor(e[j]);
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
+                    auto word = [&](int q, bool small) {
                         uint32_t v[4][4];
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             mx_unpack8(q == 0 ? d[j].x : q == 1 ? d[j].y : q == 2 ? d[j].z : d[j].w, v[j]);
+                            const uint32_t f = small ? e[j] * 0x00800080u + 129u * 0x00800080u : mx_factor(e[j]);
 #pragma unroll
-                            for (int i = 0; i < 4; i++) v[j][i] = mul_bf16x2(v[j][i], f[j]);
+                            for (int i = 0; i < 4; i++) {
+                                v[j][i] = mul_bf16x2(v[j][i], f);
+                                if (!small) v[j][i] = mx_times_rest(v[j][i], e[j]);
+                            }
                         }
-                        if (!small)
-#pragma unroll
-                            for (int j = 0; j < 4; j++)
-#pragma unroll
-                                for (int i = 0; i < 4; i++) v[j][i] = mx_times_rest(v[j][i], e[j]);
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
                             const uint4 b = xc[(n * 4 + q) * 32];
@@ -190,6 +192,13 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
                                 mma_bf16_16x8x16(sum[i][n], v[2 * i][2], v[2 * i + 1][2], v[2 * i][3], v[2 * i + 1][3], b.z, b.w);
                             }
                         }
+                    };
+                    if (__all_sync(0xffffffffu, mx_small(max(max(e[0], e[1]), max(e[2], e[3]))))) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) word(q, true);
+                    } else {
+#pragma unroll 1
+                        for (int q = 0; q < 4; q++) word(q, false);
                     }
                     s = s + 1 == RING ? 0 : s + 1;
                 }
@@ -672,6 +681,8 @@ extern "C" int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w
     if (M > 16ll * experts && experts <= TILE_MAX_EXPERTS && tile_ok(a)) return launch_tiles<true>(a, 128, 1, stream);
     return (long long)M <= 4ll * experts ? launch_stream<1>(a, experts, M < experts ? M : experts, stream) : launch_stream<2>(a, experts, M < experts ? M : experts, stream);
 }
+
+#include "gemm_mxfp4_both.cuh"
 
 // 0, or (code << 8 | role) of the first bounded wait that ran out since it was asked last
 extern "C" int fg_gemm_mxfp4_error(void) {

@@ -109,6 +109,18 @@ __device__ __forceinline__ void tc_mma_bf16_ts_pair(uint32_t d, uint32_t a, uint
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(acc) : "memory");
 }
+// D (tensor memory) (+)= A B^T of 4-bit numbers whose blocks of 32 share a power of two, 64 numbers of K; both operands in shared memory, the
+// exponents in tensor memory
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t ea, uint32_t eb, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(ea), "r"(eb), "r"(acc) : "memory");
+}
+// 512 bytes of exponents (32 rows of 16) from shared memory to four columns of tensor memory, the same for each group of 32 lanes
+__device__ __forceinline__ void tc_cp_exponents(uint32_t taddr, uint32_t saddr) {
+    const uint64_t desc = (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;      // 8 rows every 128 bytes, not swizzled
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
 // sixteen columns of this lane's row, without the wait
 __device__ __forceinline__ void tc_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "

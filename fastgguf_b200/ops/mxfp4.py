@@ -28,6 +28,8 @@ register_signatures("mx", {
                           c_void_p],
     "fg_gemm_mxfp4_grouped": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int,
                               c_void_p],
+    "fg_gemm_mxfp4_both": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p],
+    "fg_gemm_mxfp4_both_ext": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "fg_gemm_mxfp4_error": [],
 })
 
@@ -209,7 +211,13 @@ def gemm_mxfp4_both(x: Mxfp4, w: Mxfp4, *, out: Optional[torch.Tensor] = None, o
         raise KernelError("gemm_mxfp4_both: x and w are one matrix each, not stacks")
     if x.k != w.k:
         raise KernelError(f"gemm_mxfp4_both: x is {x.shape} but w is {w.shape}")
-    return gemm_mxfp4(mxfp4_rows(x, out_dtype=torch.bfloat16), w, out=out, out_dtype=out_dtype, accumulate=accumulate)
+    M = x.rows
+    out, code = _output("gemm_mxfp4_both", M, w.rows, x.device, out, out_dtype, accumulate)
+    _same_device("gemm_mxfp4_both", x.device, w.data, out)
+    with _guard(x.device):
+        check(lib("mx").fg_gemm_mxfp4_both(x.data.data_ptr(), x.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code,
+                                           out.stride(0), int(accumulate), M, w.rows, w.k, stream()), "gemm_mxfp4_both")
+    return out
 
 
 def gemm_mxfp4_grouped(x: torch.Tensor, w: Mxfp4, offsets: torch.Tensor, *, out: Optional[torch.Tensor] = None,

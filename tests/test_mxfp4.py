@@ -398,6 +398,22 @@ def test_activations_of_any_range(m, n, k):
     assert (got[0] == 0).all() and (got[:, 3] == 0).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,bn,splits", [(1, 100, 32, 16, 1), (1, 128, 64, 16, 1), (5, 129, 128, 48, 1), (100, 130, 160, 112, 1), (128, 128, 256, 128, 1), (200, 500, 288, 208, 1),
+                                             (256, 256, 512, 256, 1), (300, 384, 2080, 128, 1), (300, 384, 2080, 256, 1), (70, 300, 2048, 80, 3), (40, 100, 4096, 48, 8),
+                                             (777, 1000, 1056, 256, 2), (2048, 4096, 1024, 256, 1), (1500, 5000, 96, 128, 1)])
+def test_two_quantised_operands_at_every_width(m, n, k, bn, splits):
+    w, numbers = _matrix(n, k, n)
+    xm, xn = _matrix(m, k, m + 1, low=110, high=132)
+    want = (xn.cuda() @ numbers.cuda().T).cpu()
+    slack = (xn.cuda().abs() @ numbers.cuda().abs().T).cpu() * (2 * k / 16 + 32) * 2.0 ** -23
+    out = torch.full((m, n + 2), 7.0, device="cuda")
+    code = ops.lib("mx").fg_gemm_mxfp4_both_ext(xm.data.data_ptr(), xm.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out[:, 1:].data_ptr(), 0,
+                                                n + 2, 0, m, n, k, bn, splits, torch.cuda.current_stream().cuda_stream)
+    assert code == 0 and (out[:, 0] == 7).all() and (out[:, n + 1:] == 7).all()
+    plain.check(out[:, 1:n + 1], want, slack)
+
+
 def _runs(counts, before=0):
     return torch.tensor([before + sum(counts[:i]) for i in range(len(counts) + 1)], dtype=torch.int32)
 
