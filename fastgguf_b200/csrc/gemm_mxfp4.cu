@@ -82,6 +82,8 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
     const int c_begin = blockIdx.z * a.chunks_per_split, c_end = min(tiles_k, c_begin + a.chunks_per_split);
     const bool in_parts = c_end - c_begin > STREAM_CHUNKS(NT);
     const uint8_t *w = a.w, *sc = a.sc;
+    pdl_wait();
+    pdl_launch_dependents();
     int m_begin, m_end;
     if (a.offsets) {
         const int e = blockIdx.y;
@@ -230,8 +232,13 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
                 cluster_sync_all();
                 const uint32_t red0 = smem_u32(red);
                 for (int q = blockIdx.z * 32 * STREAM_WARPS + tid; q < total; q += 32 * STREAM_WARPS * S) {
-                    float v = 0.f;
-                    for (int z = 0; z < S; z++) v += ld_dsmem_f32(red0 + q * 4, z);
+                    float part[8];
+#pragma unroll
+                    for (int z = 0; z < 8; z++) part[z] = z < S ? ld_dsmem_f32(red0 + q * 4, z) : 0.f;
+                    float v = part[0];
+#pragma unroll
+                    for (int z = 1; z < 8; z++)
+                        if (z < S) v += part[z];
                     store(q, v);
                 }
                 cluster_sync_all();                                   // nobody overwrites or leaves what others still read
@@ -258,13 +265,7 @@ static int launch_stream(MxGemm a, int y, int busy /* of the y, that have rows *
     const int pairs = (units + STREAM_GROUPS - 1) / STREAM_GROUPS;
     int gx = room / (busy * S);                                      // as many CTAs as fit at once
     gx = gx < 1 ? 1 : gx > pairs ? pairs : gx;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(gx, y, S); cfg.blockDim = dim3(STREAM_THREADS); cfg.dynamicSmemBytes = fixed + staged * NT * 2048; cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
-    cfg.attrs = attr; cfg.numAttrs = S > 1 ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, mxfp4_stream_kernel<NT>, a, units);
+    return mx_launch(mxfp4_stream_kernel<NT>, dim3(gx, y, S), STREAM_THREADS, fixed + staged * NT * 2048, dim3(1, 1, S), stream, a, units);
 }
 
 // ---------------------------------------------------------------------------- more rows: weights through tensor memory
@@ -328,6 +329,26 @@ __device__ __forceinline__ MxTile mx_tile(const MxTiles &a, const int *cum, int 
     return t;
 }
 
+// What a CTA of a cluster that splits K stores of a tile: the columns rank, rank + S, .. below `count`, summed over the CTAs' partial tiles
+// [column][128 rows] at `part` in their shared memory, in rank order.  A thread takes four rows of a column; the CTAs' parts are asked for together.
+__device__ __forceinline__ void cluster_columns(const MxGemm &a, uint32_t part, int m0, int count, int n0, int S, int thread, int threads) {
+    const int r = (thread & 31) * 4;
+    for (int c = blockIdx.z + S * (thread >> 5); c < count; c += S * (threads >> 5)) {
+        float4 v[8];
+#pragma unroll
+        for (int z = 0; z < 8; z++)
+            if (z < S) v[z] = ld_dsmem_f32x4(part + (c * 128 + r) * 4, z);
+        float4 t = v[0];
+#pragma unroll
+        for (int z = 1; z < 8; z++)
+            if (z < S) { t.x += v[z].x; t.y += v[z].y; t.z += v[z].z; t.w += v[z].w; }
+        const float o[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (n0 + r + j < a.N) mx_store(a, m0 + c, n0 + r + j, o[j]);
+    }
+}
+
 // Sixteen columns (tokens m0 ..) of this thread's weight row n
 __device__ __forceinline__ void tile_store(const MxGemm &a, int m0, int m_end, int n, const uint32_t (&v)[16]) {
     const int count = min(16, m_end - m0);
@@ -378,6 +399,8 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x == 64) { tma_prefetch_map(&tmX); tma_prefetch_map(&tmW); }
+    pdl_wait();                                     // (before tensor memory is allocated: no kernel in front holds any then)
+    pdl_launch_dependents();
     if (warp == 1) { if (PAIR) tc_alloc_pair(smem_u32(&tmem_base_s), 512); else tc_alloc(smem_u32(&tmem_base_s), 512); }
     if (a.g.offsets && warp == 0) {                 // tiles of x in front of each expert's run
         int sum = 0;
@@ -494,6 +517,7 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                 ok = mbar_wait_warp(done0 + 8 * set, (stage / TILE_SLOTS - 1) & 1);
                 if (!ok) { mx_raise(7); return; }
             }
+            __syncwarp();
             tc_fence_after();
 #pragma unroll
             for (int q = 0; q < 4; q++) {           // a block of 32 numbers
@@ -508,11 +532,13 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                 if (PAIR) mbar_arrive_cluster(full + 8 * set); else mbar_arrive(full + 8 * set);
                 mbar_arrive(wempty0 + 8 * s);
             }
+            __syncwarp();                           // (tcgen05.st and ld want a converged warp)
         };
         auto epilogue = [&](int T) {
             const MxTile t = mx_tile<PAIR>(a, cum, T, rank);
             const bool have = mbar_wait_warp(tfull, i & 1);
             if (!have) { mx_raise(5); ok = false; }
+            __syncwarp();
             tc_fence_after();
             uint32_t v[4][16];                      // columns 16 (4 q + set) ..
 #pragma unroll
@@ -522,6 +548,7 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
             tc_fence_before();
             __syncwarp();
             if (lane == 0) { if (PAIR) mbar_arrive_cluster(empty); else mbar_arrive(empty); }
+            __syncwarp();
             if (!PAIR && S > 1) {
                 float *part = (float *)smem;        // [bn][128]: the rings are idle
 #pragma unroll
@@ -558,12 +585,7 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         cluster_sync_all();
         if (warp >= 3) {
             const MxTile t = mx_tile<PAIR>(a, cum, first, rank);
-            const int r = (threadIdx.x - 96) & 127, n = t.n0 + r;
-            for (int c = blockIdx.z + S * ((threadIdx.x - 96) >> 7); c < min(bn, t.m_end - t.m0); c += 4 * S) {
-                float v = 0.f;
-                for (int z = 0; z < S; z++) v += ld_dsmem_f32(smem0 + (c * TILE_ROWS + r) * 4, z);
-                if (n < a.g.N) mx_store(a.g, t.m0 + c, n, v);
-            }
+            cluster_columns(a.g, smem0, t.m0, min(bn, t.m_end - t.m0), t.n0, S, threadIdx.x - 96, 512);
         }
         cluster_sync_all();                         // nobody leaves while others read its shared memory
     }
@@ -601,14 +623,7 @@ static int launch_tiles(const MxGemm &g, int bn, int S, cudaStream_t stream) {
     }
     const int units = PAIR ? mx_sm_count() / 2 : mx_sm_count();
     const unsigned gx = S > 1 || tiles < units ? (unsigned)tiles : (unsigned)units;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(PAIR ? 2 * gx : gx, 1, S);
-    cfg.blockDim = dim3(TILE_THREADS); cfg.dynamicSmemBytes = TILE_SMEM; cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = PAIR ? 2 : 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
-    cfg.attrs = attr; cfg.numAttrs = PAIR || S > 1 ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, mxfp4_tile_kernel<PAIR>, tmX, tmW, a);
+    return mx_launch(mxfp4_tile_kernel<PAIR>, dim3(PAIR ? 2 * gx : gx, 1, S), TILE_THREADS, TILE_SMEM, dim3(PAIR ? 2 : 1, 1, S), stream, tmX, tmW, a);
 }
 // whether TMA can bring the rows of x
 static bool tile_ok(const MxGemm &g) { return g.x_vec && g.ldx >= g.K; }

@@ -50,6 +50,8 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x == 64) { tma_prefetch_map(&tmX); tma_prefetch_map(&tmW); }
+    pdl_wait();                                     // (before tensor memory is allocated: no kernel in front holds any then)
+    pdl_launch_dependents();
     if (warp == 1) tc_alloc(smem_u32(&tmem_base_s), 512);
     tc_fence_before();
     __syncthreads();
@@ -125,6 +127,7 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
             const int m0 = T % a.tiles_m * bn, n = T / a.tiles_m * BOTH_ROWS + r;
             const bool have = mbar_wait_warp(tfull, i & 1);
             if (!have) mx_raise(5);
+            __syncwarp();
             tc_fence_after();
             uint32_t v[8][16];                      // columns 16 (2 q + half) ..
 #pragma unroll
@@ -134,6 +137,7 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(tempty);
+            __syncwarp();                           // (tcgen05.ld wants a converged warp)
             if (S > 1) {
                 float *part = (float *)smem;        // [bn][128]: the ring is idle
 #pragma unroll
@@ -154,12 +158,8 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         // the columns rank, rank + S, .. of the tile: partial sums of all CTAs of the cluster, in rank order
         cluster_sync_all();
         if (warp >= 2) {
-            const int m0 = (int)blockIdx.x % a.tiles_m * bn, r = (threadIdx.x - 64) & 127, n = (int)blockIdx.x / a.tiles_m * BOTH_ROWS + r;
-            for (int c = blockIdx.z + S * ((threadIdx.x - 64) >> 7); c < min(bn, a.g.M - m0); c += 2 * S) {
-                float v = 0.f;
-                for (int z = 0; z < S; z++) v += ld_dsmem_f32(smem0 + (c * BOTH_ROWS + r) * 4, z);
-                if (n < a.g.N) mx_store(a.g, m0 + c, n, v);
-            }
+            const int m0 = (int)blockIdx.x % a.tiles_m * bn;
+            cluster_columns(a.g, smem0, m0, min(bn, a.g.M - m0), (int)blockIdx.x / a.tiles_m * BOTH_ROWS, S, threadIdx.x - 64, 256);
         }
         cluster_sync_all();                         // nobody leaves while others read its shared memory
     }
@@ -192,15 +192,8 @@ static int launch_both(MxBoth a, const void *x, int bn, int S, cudaStream_t stre
         if (e != cudaSuccess) return (int)e;
     }
     const int n_sm = mx_sm_count();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(S > 1 || tiles < n_sm ? (unsigned)tiles : (unsigned)n_sm, 1, S);
     // (all of an SM's shared memory, needed or not: see launch_tiles)
-    cfg.blockDim = dim3(BOTH_THREADS); cfg.dynamicSmemBytes = BOTH_SMEM; cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
-    cfg.attrs = attr; cfg.numAttrs = S > 1 ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, mxfp4_both_kernel, tmX, tmW, a);
+    return mx_launch(mxfp4_both_kernel, dim3(S > 1 || tiles < n_sm ? (unsigned)tiles : (unsigned)n_sm, 1, S), BOTH_THREADS, BOTH_SMEM, dim3(1, 1, S), stream, tmX, tmW, a);
 }
 
 // The tile's width and the split of K that finish first: rounds of tiles over the SMs times what a tile takes, in SM cycles.  Tiles of

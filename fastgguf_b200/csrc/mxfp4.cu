@@ -48,6 +48,8 @@ mxfp4_quantize_kernel(const T *__restrict__ x, long long ldx, long long x_stride
     const int tk = blockIdx.x, tr = blockIdx.y % tiles_r, mat = blockIdx.y / tiles_r, tiles_k = gridDim.x;
     const int c = threadIdx.x & 15, k = tk * 128 + c * 8, rows = min(128, R - tr * 128);
     if (threadIdx.x < 32) ((uint4 *)tile)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    pdl_wait();
+    pdl_launch_dependents();
     __syncthreads();
     const T *src = x + (size_t)mat * x_stride + k;
     uint8_t *dst = data + (size_t)mat * R * (K / 2) + k / 2;
@@ -98,8 +100,8 @@ extern "C" int fg_mxfp4_quantize(const void *x, int dtype, long long ldx, long l
     const int vec = ((uintptr_t)x & 15) == 0 && (ldx * size) % 16 == 0 && (x_stride * size) % 16 == 0;
     dim3 grid(mx_tiles(K), tiles_r * mats);
     if (dtype == FG_F32)
-        return fg_launch_in_order(mxfp4_quantize_kernel<float>, grid, dim3(256), 0, stream, (const float *)x, ldx, x_stride, (uint8_t *)data, (uint8_t *)scales, R, K, tiles_r, vec);
-    return fg_launch_in_order(mxfp4_quantize_kernel<bf16>, grid, dim3(256), 0, stream, (const bf16 *)x, ldx, x_stride, (uint8_t *)data, (uint8_t *)scales, R, K, tiles_r, vec);
+        return mx_launch(mxfp4_quantize_kernel<float>, grid, 256, 0, dim3(1, 1, 1), stream, (const float *)x, ldx, x_stride, (uint8_t *)data, (uint8_t *)scales, R, K, tiles_r, vec);
+    return mx_launch(mxfp4_quantize_kernel<bf16>, grid, 256, 0, dim3(1, 1, 1), stream, (const bf16 *)x, ldx, x_stride, (uint8_t *)data, (uint8_t *)scales, R, K, tiles_r, vec);
 }
 
 // ---------------------------------------------------------------------------- rows
@@ -111,6 +113,7 @@ mxfp4_rows_kernel(const uint8_t *__restrict__ data, const uint8_t *__restrict__ 
                   long long ldo, long long total, int R, int K, float scale, int vec) {
     constexpr int V = 16 / sizeof(T);
     const int per_row = K / V, tiles_k = mx_tiles(K);
+    pdl_wait();
     for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long long)gridDim.x * 256) {
         const long long i = at / per_row;
         const int c = (int)(at - i * per_row) * V;
@@ -159,6 +162,6 @@ extern "C" int fg_mxfp4_rows(const void *data, const void *scales, const int *ro
     const long long total = (long long)n * (K / V), want = (total + 255) / 256;
     dim3 grid((unsigned)(want < 148 * 64 ? want : 148 * 64));
     if (out_dtype == FG_F32)
-        return fg_launch_in_order(mxfp4_rows_kernel<float>, grid, dim3(256), 0, stream, (const uint8_t *)data, (const uint8_t *)scales, rows, (float *)out, ldo, total, R, K, scale, vec);
-    return fg_launch_in_order(mxfp4_rows_kernel<bf16>, grid, dim3(256), 0, stream, (const uint8_t *)data, (const uint8_t *)scales, rows, (bf16 *)out, ldo, total, R, K, scale, vec);
+        return mx_launch(mxfp4_rows_kernel<float>, grid, 256, 0, dim3(1, 1, 1), stream, (const uint8_t *)data, (const uint8_t *)scales, rows, (float *)out, ldo, total, R, K, scale, vec);
+    return mx_launch(mxfp4_rows_kernel<bf16>, grid, 256, 0, dim3(1, 1, 1), stream, (const uint8_t *)data, (const uint8_t *)scales, rows, (bf16 *)out, ldo, total, R, K, scale, vec);
 }

@@ -63,3 +63,26 @@ __device__ __forceinline__ void mx_unpack32(const uint4 &d, uint32_t e, uint32_t
         for (int j = 0; j < 16; j++) out[j] = mx_times_rest(out[j], e);
     }
 }
+
+// ---------------------------------------------------------------------------- launches
+// Dependent launches: a kernel of this library waits for its predecessor before it touches any memory (weights too: the quantiser may just have
+// written them) and only then releases its successor, so that one never runs beside the kernel before its predecessor.  The release
+// saves the drain and the launch between two small kernels.  mxfp4_rows, whose output may be weights that a contraction reads before its wait, does not
+// release early.
+template <typename... KArgs, typename... Args>
+static inline int mx_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, dim3 cluster, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (fg_pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster.x * cluster.y * cluster.z > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster.x; attr[n].val.clusterDim.y = cluster.y; attr[n++].val.clusterDim.z = cluster.z;
+    }
+    cfg.attrs = attr; cfg.numAttrs = n;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}

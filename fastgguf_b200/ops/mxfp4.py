@@ -12,13 +12,12 @@ A number is a sign, two exponent bits and one mantissa bit (0, 0.5, 1, 1.5, 2, 3
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
 import torch
 
-from .lib import FG_BF16, FG_F32, KernelError, check, lib, register_signatures, require_cuda, stream
+from .lib import FG_BF16, FG_F32, KernelError, check, lib, register_signatures, require_cuda
 
 register_signatures("mx", {
     "fg_mxfp4_quantize": [c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
@@ -99,9 +98,20 @@ class Mxfp4:
         return full[..., :self.rows, :self.k // BLOCK].contiguous()
 
 
-def _guard(device: torch.device):
-    """Launches go to the tensors' device, whichever is current."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+_launchers: dict = {}
+
+
+def _launch(name: str, device: int, *args) -> None:
+    """Calls a launcher on the tensors' device, whichever is current, and that device's current stream.  (A small step's time is the host's: what a call
+    needs is looked up once.)"""
+    fn = _launchers.get(name)
+    if fn is None:
+        fn = _launchers[name] = getattr(lib("mx"), "fg_" + name)
+    if device == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device)), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(device)), name)
 
 
 def _same_device(what: str, device: torch.device, *tensors) -> None:
@@ -134,12 +144,13 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
     if x.stride(-1) != 1:
         raise KernelError("mxfp4_quantize: the numbers of a row must be contiguous")
     lead = x.shape[:-2]
-    data = torch.empty((*lead, rows, k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*lead, *_scale_shape(rows, k)), dtype=torch.uint8, device=x.device)
-    with _guard(x.device):
-        check(lib("mx").fg_mxfp4_quantize(x.data_ptr(), code, x.stride(-2), x.stride(0) if lead else 0, data.data_ptr(), scales.data_ptr(),
-                                          lead[0] if lead else 1, rows, k, stream()), "mxfp4_quantize")
-    return Mxfp4(data, scales)
+    q = Mxfp4.__new__(Mxfp4)                     # (as its constructor would leave it)
+    q.rows, q.k = rows, k
+    q.data = data = x.new_empty((*lead, rows, k // 2), dtype=torch.uint8)
+    q.scales = scales = x.new_empty((*lead, *_scale_shape(rows, k)), dtype=torch.uint8)
+    _launch("mxfp4_quantize", x.get_device(), x.data_ptr(), code, x.stride(-2), x.stride(0) if lead else 0, data.data_ptr(), scales.data_ptr(),
+            lead[0] if lead else 1, rows, k)
+    return q
 
 
 def mxfp4_rows(w: Mxfp4, rows: Optional[torch.Tensor] = None, *, scale: float = 1.0, out: Optional[torch.Tensor] = None,
@@ -153,22 +164,21 @@ def mxfp4_rows(w: Mxfp4, rows: Optional[torch.Tensor] = None, *, scale: float = 
         raise KernelError(f"mxfp4_rows: rows must be a contiguous int32 vector, got {rows.dtype} {tuple(rows.shape)}")
     n = w.rows if rows is None else rows.numel()
     if out is None:
-        out = torch.empty((n, w.k), dtype=out_dtype or torch.float32, device=w.device)
+        out = w.data.new_empty((n, w.k), dtype=out_dtype or torch.float32)
     elif out.shape != (n, w.k) or out.stride(1) != 1 or (n > 1 and out.stride(0) < w.k) or (out_dtype is not None and out.dtype != out_dtype):
         raise KernelError(f"mxfp4_rows: out must be [{n}, {w.k}] with contiguous rows")
     code = _out_code("mxfp4_rows", out.dtype)
     _same_device("mxfp4_rows", w.device, rows, out)
-    with _guard(w.device):
-        check(lib("mx").fg_mxfp4_rows(w.data.data_ptr(), w.scales.data_ptr(), rows.data_ptr() if rows is not None else None, out.data_ptr(), code,
-                                      max(out.stride(0), w.k), n, w.rows, w.k, float(scale), stream()), "mxfp4_rows")
+    _launch("mxfp4_rows", out.get_device(), w.data.data_ptr(), w.scales.data_ptr(), rows.data_ptr() if rows is not None else None, out.data_ptr(), code,
+            max(out.stride(0), w.k), n, w.rows, w.k, scale)
     return out
 
 
-def _output(what: str, M: int, N: int, device: torch.device, out, out_dtype, accumulate: bool) -> tuple:
+def _output(what: str, M: int, N: int, like: torch.Tensor, out, out_dtype, accumulate: bool) -> tuple:
     if out is None:
         if accumulate:
             raise KernelError(f"{what}: accumulate needs the tensor to accumulate into")
-        out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=device)
+        out = like.new_empty((M, N), dtype=out_dtype or torch.bfloat16)
     elif out.shape != (M, N) or out.stride(1) != 1 or (M > 1 and out.stride(0) < N) or (out_dtype is not None and out.dtype != out_dtype):
         raise KernelError(f"{what}: out must be [{M}, {N}] with contiguous rows")
     code = _out_code(what, out.dtype)
@@ -195,11 +205,10 @@ def gemm_mxfp4(x: torch.Tensor, w: Mxfp4, *, out: Optional[torch.Tensor] = None,
         raise KernelError("gemm_mxfp4: w is one matrix, not a stack (see gemm_mxfp4_grouped)")
     _activations("gemm_mxfp4", x, w.k)
     M = x.shape[0]
-    out, code = _output("gemm_mxfp4", M, w.rows, x.device, out, out_dtype, accumulate)
+    out, code = _output("gemm_mxfp4", M, w.rows, w.data, out, out_dtype, accumulate)
     _same_device("gemm_mxfp4", x.device, w.data, out)
-    with _guard(x.device):
-        check(lib("mx").fg_gemm_mxfp4(x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, out.stride(0),
-                                      int(accumulate), M, w.rows, w.k, stream()), "gemm_mxfp4")
+    _launch("gemm_mxfp4", x.get_device(), x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, out.stride(0),
+            accumulate, M, w.rows, w.k)
     return out
 
 
@@ -212,11 +221,10 @@ def gemm_mxfp4_both(x: Mxfp4, w: Mxfp4, *, out: Optional[torch.Tensor] = None, o
     if x.k != w.k:
         raise KernelError(f"gemm_mxfp4_both: x is {x.shape} but w is {w.shape}")
     M = x.rows
-    out, code = _output("gemm_mxfp4_both", M, w.rows, x.device, out, out_dtype, accumulate)
+    out, code = _output("gemm_mxfp4_both", M, w.rows, w.data, out, out_dtype, accumulate)
     _same_device("gemm_mxfp4_both", x.device, w.data, out)
-    with _guard(x.device):
-        check(lib("mx").fg_gemm_mxfp4_both(x.data.data_ptr(), x.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code,
-                                           out.stride(0), int(accumulate), M, w.rows, w.k, stream()), "gemm_mxfp4_both")
+    _launch("gemm_mxfp4_both", out.get_device(), x.data.data_ptr(), x.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code,
+            out.stride(0), accumulate, M, w.rows, w.k)
     return out
 
 
@@ -234,9 +242,8 @@ def gemm_mxfp4_grouped(x: torch.Tensor, w: Mxfp4, offsets: torch.Tensor, *, out:
         raise KernelError(f"gemm_mxfp4_grouped: offsets must be contiguous int32 [{X + 1}], got {offsets.dtype} {tuple(offsets.shape)}")
     _activations("gemm_mxfp4_grouped", x, w.k)
     M = x.shape[0]
-    out, code = _output("gemm_mxfp4_grouped", M, w.rows, x.device, out, out_dtype, accumulate)
+    out, code = _output("gemm_mxfp4_grouped", M, w.rows, w.data, out, out_dtype, accumulate)
     _same_device("gemm_mxfp4_grouped", x.device, w.data, offsets, out)
-    with _guard(x.device):
-        check(lib("mx").fg_gemm_mxfp4_grouped(x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), offsets.data_ptr(), X, out.data_ptr(),
-                                              code, out.stride(0), int(accumulate), M, w.rows, w.k, stream()), "gemm_mxfp4_grouped")
+    _launch("gemm_mxfp4_grouped", x.get_device(), x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), offsets.data_ptr(), X, out.data_ptr(),
+            code, out.stride(0), accumulate, M, w.rows, w.k)
     return out

@@ -71,15 +71,11 @@ def test_there_is_no_cpu_path():
             call()
 
 
-class _OnDevice:
-    """Stands for tensors on a device where only the checks in front of the launch are looked at."""
-
-
 @pytest.fixture
 def no_device_check(monkeypatch):
     from fastgguf_b200.ops import mxfp4
     monkeypatch.setattr(mxfp4, "require_cuda", lambda *t: None)
-    monkeypatch.setattr(mxfp4, "lib", lambda *a: pytest.fail("a refused call reached a kernel"))
+    monkeypatch.setattr(mxfp4, "_launch", lambda *a: pytest.fail("a refused call reached a kernel"))
 
 
 def test_calls_that_do_not_fit_are_refused_before_a_launch(no_device_check):
