@@ -250,20 +250,22 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
 
 template <int NT>
 static int launch_stream(MxGemm a, int y, int busy /* of the y, that have rows */, cudaStream_t stream) {
-    const int tiles_k = mx_tiles(a.K), units = 4 * mx_tiles(a.N), room = mx_sm_count();
-    // K over a cluster: until x fits at once, and while there are too few units for the SMs and each warp keeps a chunk
-    int S = 1;
-    while (S < 8 && (tiles_k > S * STREAM_CHUNKS(NT) || ((long long)units * busy * S <= room * STREAM_GROUPS / 2 && tiles_k > S * STREAM_WARPS))) S *= 2;
-    a.chunks_per_split = (tiles_k + S - 1) / S;
-    const int staged = a.chunks_per_split < STREAM_CHUNKS(NT) ? a.chunks_per_split : STREAM_CHUNKS(NT);
     constexpr int fixed = STREAM_GROUPS * STREAM_WARPS * (STREAM_RING(NT) * STREAM_SLOT + 8 * NT * STREAM_ROWS * 4);
     static FgPerDevice configured;
     if (fg_needs_setup(configured)) {
         cudaError_t e = cudaFuncSetAttribute(mxfp4_stream_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + 65536);
         if (e != cudaSuccess) return (int)e;
     }
+    static MxClusters known;
+    auto room = [&](int S) { return mx_clusters(known, mxfp4_stream_kernel<NT>, STREAM_THREADS, fixed + 65536, S); };
+    const int tiles_k = mx_tiles(a.K), units = 4 * mx_tiles(a.N);
+    // K over a cluster: until x fits at once, and while there are too few units for the SMs and each warp keeps a chunk
+    int S = 1;
+    while (S < 8 && (tiles_k > S * STREAM_CHUNKS(NT) || ((long long)units * busy <= room(2 * S) * STREAM_GROUPS && tiles_k > S * STREAM_WARPS))) S *= 2;
+    a.chunks_per_split = (tiles_k + S - 1) / S;
+    const int staged = a.chunks_per_split < STREAM_CHUNKS(NT) ? a.chunks_per_split : STREAM_CHUNKS(NT);
     const int pairs = (units + STREAM_GROUPS - 1) / STREAM_GROUPS;
-    int gx = room / (busy * S);                                      // as many CTAs as fit at once
+    int gx = room(S) / busy;                                         // as many CTAs as fit at once
     gx = gx < 1 ? 1 : gx > pairs ? pairs : gx;
     return mx_launch(mxfp4_stream_kernel<NT>, dim3(gx, y, S), STREAM_THREADS, fixed + staged * NT * 2048, dim3(1, 1, S), stream, a, units);
 }
@@ -295,7 +297,7 @@ static int launch_stream(MxGemm a, int y, int busy /* of the y, that have rows *
 #define TILE_AHEAD 3            // stages of the next tile that are unpacked before a tile's epilogue
 #define TILE_MAX_EXPERTS 1024
 #define TILE_SMEM (221 * 1024)
-#define TILE_UNPACK 520         // SM cycles that unpacking a stage takes at least (the integer pipe's)
+#define TILE_UNPACK 650         // SM cycles a stage takes at few tokens: its unpacking
 
 struct MxTiles {
     MxGemm g;
@@ -597,6 +599,12 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
 }
 
 template <bool PAIR>
+static int tile_setup() {
+    static FgPerDevice configured;
+    return fg_needs_setup(configured) ? (int)cudaFuncSetAttribute(mxfp4_tile_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM) : 0;
+}
+
+template <bool PAIR>
 static int launch_tiles(const MxGemm &g, int bn, int S, cudaStream_t stream) {
     MxTiles a;
     a.g = g; a.bn = bn;
@@ -616,11 +624,8 @@ static int launch_tiles(const MxGemm &g, int bn, int S, cudaStream_t stream) {
     if (rc) return rc;
     // All of an SM's shared memory, needed or not: a CTA that allocates tensor memory shares its SM with no other that does (of a kernel on
     // another stream, say), whose cluster might wait for one of this kernel's while it waits for tensor memory.
-    static FgPerDevice configured;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(mxfp4_tile_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM);
-        if (e != cudaSuccess) return (int)e;
-    }
+    rc = tile_setup<PAIR>();
+    if (rc) return rc;
     const int units = PAIR ? mx_sm_count() / 2 : mx_sm_count();
     const unsigned gx = S > 1 || tiles < units ? (unsigned)tiles : (unsigned)units;
     return mx_launch(mxfp4_tile_kernel<PAIR>, dim3(PAIR ? 2 * gx : gx, 1, S), TILE_THREADS, TILE_SMEM, dim3(PAIR ? 2 : 1, 1, S), stream, tmX, tmW, a);
@@ -628,10 +633,14 @@ static int launch_tiles(const MxGemm &g, int bn, int S, cudaStream_t stream) {
 // whether TMA can bring the rows of x
 static bool tile_ok(const MxGemm &g) { return g.x_vec && g.ldx >= g.K; }
 
-// The form, the tile's width and the split of K that finish first: rounds of tiles over the SMs times what a tile takes, in SM cycles - a
-// stage the longer of its MMAs (4 BN) and its unpacking, and once a tile its start and epilogue.
-static void tile_plan(int M, int N, int K, int n_sm, bool &pair, int &bn, int &S) {
-    const int tiles_k = mx_tiles(K);
+// The form, the tile's width and the split of K that finish first, in SM cycles.  A stage takes the longer of its unpacking and its MMAs, as
+// measured at both ends (pairs: 820 cycles at 128 tokens, 1,350 at 256; single CTAs, bound by the bytes an SM receives: 950 and 1,690).  Half of a
+// step counts whole rounds of tiles over the SMs, half the tiles alone: at the power limit the clock rises while SMs are idle (2,048 x 14,336 x 4,096 in
+// seven rounds of 256 tokens takes 161 to 180 us, in the ten of 160 tokens, 7 % fewer by rounds, 192).
+static void tile_plan(int M, int N, int K, bool &pair, int &bn, int &S) {
+    static MxClusters known;
+    const int tiles_k = mx_tiles(K), n_sm = mx_sm_count();
+    if (tile_setup<false>()) cudaGetLastError();                     // (its launch reports it)
     double best = 1e30;
     for (int p = 0; p < 2; p++) {
         const int rows = p ? 2 * TILE_ROWS : TILE_ROWS, tiles_n = (N + rows - 1) / rows, units = p ? n_sm / 2 : n_sm;
@@ -639,11 +648,13 @@ static void tile_plan(int M, int N, int K, int n_sm, bool &pair, int &bn, int &S
             if (b > 16 && b - 16 >= M) break;                        // wider than the rows there are
             const long long tiles = (long long)((M + b - 1) / b) * tiles_n;
             for (int s = 1; s <= (p ? 1 : 8); s++) {
-                if (s > 1 && tiles * s > units) break;
+                if (s > 1 && tiles > mx_clusters(known, mxfp4_tile_kernel<false>, TILE_THREADS, TILE_SMEM, s)) continue;
                 const int kb = (tiles_k + s - 1) / s;
-                const double mma = (p ? 4.0 : 5.0) * b, stage = mma > TILE_UNPACK ? mma : TILE_UNPACK;
-                const double tile = kb * stage + 2500 + 4.0 * b + (s > 1 ? 1500 + 12.0 * b : 0);
-                const double cost = (double)((tiles * s + units - 1) / units) * tile;
+                const double mma = p ? 300 + 4.1 * b : 210 + 5.8 * b, stage = mma > TILE_UNPACK ? mma : TILE_UNPACK;
+                const double tile = kb * stage + 2500 + 4.0 * b + (s > 1 ? 2500 + 8.0 * b : 0);
+                const long long rounds = (tiles * s + units - 1) / units;
+                const double even = (double)(tiles * s) / units;
+                const double cost = (rounds > 1 ? 0.5 * (rounds + even) : 1.0) * tile;
                 if (cost < best) { best = cost; pair = p; bn = b; S = s; }
             }
         }
@@ -668,8 +679,8 @@ extern "C" int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, co
     a.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     if (form == 0) {
         bool pair = false;
-        form = M > 16 && tile_ok(a) ? 2 : 1;
-        if (form == 2) tile_plan(M, N, K, mx_sm_count(), pair, bn, splits);
+        form = M > 8 && tile_ok(a) ? 2 : 1;
+        if (form == 2) tile_plan(M, N, K, pair, bn, splits);
         if (pair) form = 3;
     } else if (form < 1 || form > 3 || (form > 1 && (!tile_ok(a) || bn < 16 || bn > 256 || bn % 16 || splits < 1 || splits > 8 || (form == 3 && splits > 1))))
         return FG_ERR_BAD_SIZE;

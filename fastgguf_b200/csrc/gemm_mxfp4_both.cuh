@@ -168,6 +168,11 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     if (warp == 1) { tc_fence_after(); tc_free(tmem, 512); }
 }
 
+static int both_setup() {
+    static FgPerDevice configured;
+    return fg_needs_setup(configured) ? (int)cudaFuncSetAttribute(mxfp4_both_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BOTH_SMEM) : 0;
+}
+
 static int launch_both(MxBoth a, const void *x, int bn, int S, cudaStream_t stream) {
     const MxGemm &g = a.g;
     const int all_kb = (g.K + BOTH_K - 1) / BOTH_K, sides = bn > 128 ? 2 : 1;
@@ -186,11 +191,8 @@ static int launch_both(MxBoth a, const void *x, int bn, int S, cudaStream_t stre
     if (rc) return rc;
     rc = mx_make_map(&tmW, g.w, false, g.N, g.K / 2, g.K / 2, BOTH_ROWS, BOTH_K / 2, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
-    static FgPerDevice configured;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(mxfp4_both_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BOTH_SMEM);
-        if (e != cudaSuccess) return (int)e;
-    }
+    rc = both_setup();
+    if (rc) return rc;
     const int n_sm = mx_sm_count();
     // (all of an SM's shared memory, needed or not: see launch_tiles)
     return mx_launch(mxfp4_both_kernel, dim3(S > 1 || tiles < n_sm ? (unsigned)tiles : (unsigned)n_sm, 1, S), BOTH_THREADS, BOTH_SMEM, dim3(1, 1, S), stream, tmX, tmW, a);
@@ -198,15 +200,17 @@ static int launch_both(MxBoth a, const void *x, int bn, int S, cudaStream_t stre
 
 // The tile's width and the split of K that finish first: rounds of tiles over the SMs times what a tile takes, in SM cycles.  Tiles of
 // more than one start at multiples of 128 tokens, where tiles of exponents do.
-static void both_plan(int M, int N, int K, int n_sm, int &bn, int &S) {
-    const int all_kb = (K + BOTH_K - 1) / BOTH_K, tiles_n = mx_tiles(N), whole = (M + 15) / 16 * 16;
-    const int widths[3] = {whole < 256 ? whole : 256, whole < 128 ? whole : 128, whole < 256 ? whole : 256};
+static void both_plan(int M, int N, int K, int &bn, int &S) {
+    static MxClusters known;
+    if (both_setup()) cudaGetLastError();                            // (its launch reports it)
+    const int n_sm = mx_sm_count(), all_kb = (K + BOTH_K - 1) / BOTH_K, tiles_n = mx_tiles(N), whole = (M + 15) / 16 * 16;
+    const int widths[2] = {whole < 256 ? whole : 256, whole < 128 ? whole : 128};
     double best = 1e30;
     for (int i = 0; i < 2; i++) {
         const int b = widths[i];
         const long long tiles = (long long)((M + b - 1) / b) * tiles_n;
         for (int s = 1; s <= 8; s++) {
-            if (s > 1 && tiles * s > n_sm) break;
+            if (s > 1 && tiles > mx_clusters(known, mxfp4_both_kernel, BOTH_THREADS, BOTH_SMEM, s)) continue;
             const int kb = (all_kb + s - 1) / s;
             const double tile = kb * (300 + 1.9 * b) + 2500 + 5.0 * b + (s > 1 ? 1500 + 12.0 * b : 0);
             const double cost = (double)((tiles * s + n_sm - 1) / n_sm) * tile;
@@ -226,7 +230,7 @@ extern "C" int fg_gemm_mxfp4_both_ext(const void *x, const void *x_scales, const
     if (bad) return bad;
     if (((uintptr_t)x & 15) || ((uintptr_t)x_scales & 15)) return FG_ERR_BAD_SIZE;
     if (M == 0) return 0;
-    if (bn == 0) both_plan(M, N, K, mx_sm_count(), bn, splits);
+    if (bn == 0) both_plan(M, N, K, bn, splits);
     else if (bn < 16 || bn > 256 || bn % 16 || (bn % 128 && bn < M) || splits < 1 || splits > 8) return FG_ERR_BAD_SIZE;
     return launch_both(a, x, bn, splits, stream);
 }

@@ -195,3 +195,26 @@ static inline int mx_sm_count() {
     if (n[dev] == 0 && (cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n[dev] <= 0)) n[dev] = 148;
     return n[dev];
 }
+// How many clusters of S CTAs (along z; S 1: CTAs) of a kernel that takes an SM to itself run at once: clusters stay inside a group of SMs, and the groups' sizes
+// are no multiples of S (of 7 or 8, fewer than 16 fit).  Asked once per device and S.
+struct MxClusters { short n[64][9]; };
+template <typename K>
+static inline int mx_clusters(MxClusters &known, K kernel, int threads, int smem, int S) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    short &n = known.n[dev][S];
+    if (n == 0) {
+        int got = 0;
+        if (S > 1) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1, 1, S); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
+            cfg.attrs = attr; cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess) { got = 0; cudaGetLastError(); }
+        }
+        n = (short)(got > 0 ? got : mx_sm_count() / S);
+    }
+    return n;
+}
