@@ -416,6 +416,7 @@ int fg_gemm_mxfp4_both_ext(const void *x, const void *x_scales, const void *w, c
                            int accumulate, int M, int N, int K, int bn, int splits, cudaStream_t stream);
 /* 0, or (code << 8 | role) of the first bounded wait of these kernels that ran out since it was asked last */
 int fg_gemm_mxfp4_error(void);
+int fg_gemm_mxfp4_test_hook(long long wait_limit_cycles, int skip_copy);   /* tests only */
 
 #ifdef __cplusplus
 }

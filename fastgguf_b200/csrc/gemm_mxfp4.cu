@@ -303,7 +303,10 @@ struct MxTiles {
     MxGemm g;
     int bn, xs, tiles_m, tiles_n, n_tiles;          // tokens a tile, depth of their ring (grouped: tiles_m and n_tiles follow from the offsets)
     int kb_per_split;
+    int test_skip_copy;                             // tests only: the tokens of the first stage are not copied
 };
+static int g_mx_test_skip_copy = 0;                 // host side of fg_gemm_mxfp4_test_hook
+
 // a tile: rows [m0, m_end) of x, weight rows from n0 (row w_row of the stack, exponents from tile sc_tile)
 struct MxTile { int m0, m_end, n0, w_row, sc_tile; };
 
@@ -438,7 +441,9 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                 if (elect_one()) {
                     const uint32_t dst = smem0 + s * x_bytes, bar = full + 8 * slot;
                     if (rank == 0) mbar_expect_tx(full0 + 8 * slot, (PAIR ? 2 : 1) * x_bytes);
-                    if (PAIR) { tma_load_2d_pair(dst, &tmX, kb * TILE_K, m0, bar); tma_load_2d_pair(dst + x_half, &tmX, kb * TILE_K + 64, m0, bar); }
+                    // (a test may ask for the first stage to stay incomplete: its barrier then never fires and every wait runs out)
+                    if (a.test_skip_copy && g == 0) {}
+                    else if (PAIR) { tma_load_2d_pair(dst, &tmX, kb * TILE_K, m0, bar); tma_load_2d_pair(dst + x_half, &tmX, kb * TILE_K + 64, m0, bar); }
                     else { tma_load_2d(dst, &tmX, kb * TILE_K, m0, bar); tma_load_2d(dst + x_half, &tmX, kb * TILE_K + 64, m0, bar); }
                 }
                 __syncwarp();
@@ -607,7 +612,7 @@ static int tile_setup() {
 template <bool PAIR>
 static int launch_tiles(const MxGemm &g, int bn, int S, cudaStream_t stream) {
     MxTiles a;
-    a.g = g; a.bn = bn;
+    a.g = g; a.bn = bn; a.test_skip_copy = g_mx_test_skip_copy;
     const int x_bytes = (PAIR ? bn / 2 : bn) * 256, room = (TILE_SMEM - 1024 - TILE_W_STAGES * TILE_W_STAGE) / x_bytes;
     a.xs = room < TILE_SLOTS ? room : TILE_SLOTS;
     const int tiles_k = mx_tiles(g.K), rows = PAIR ? 2 * TILE_ROWS : TILE_ROWS;
@@ -716,4 +721,10 @@ extern "C" int fg_gemm_mxfp4_error(void) {
     if (cudaMemcpyFromSymbol(&v, g_mx_error, sizeof(int)) != cudaSuccess) return -1;
     if (v) cudaMemcpyToSymbol(g_mx_error, &zero, sizeof(int));
     return v;
+}
+// tests only: how long a wait may last, in SM cycles (0: the ordinary limit), and whether a kernel's first copy of tokens is left out
+extern "C" int fg_gemm_mxfp4_test_hook(long long wait_limit_cycles, int skip_copy) {
+    const long long limit = wait_limit_cycles > 0 ? wait_limit_cycles : MX_WAIT_LIMIT_CYCLES;
+    g_mx_test_skip_copy = skip_copy;
+    return (int)cudaMemcpyToSymbol(g_mx_wait_limit, &limit, sizeof(limit));
 }

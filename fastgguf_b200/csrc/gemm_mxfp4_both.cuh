@@ -24,7 +24,7 @@
 struct MxBoth {
     MxGemm g;                                       // (x, ldx, x_vec unused)
     const uint8_t *xsc;                             // exponents of x
-    int bn, stages, tiles_m, n_tiles, kb_per_split;
+    int bn, stages, tiles_m, n_tiles, kb_per_split, test_skip_copy;
 };
 
 __global__ void __launch_bounds__(BOTH_THREADS, 1)
@@ -72,7 +72,7 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                     const int halves = min(2, tiles_k - 2 * kb);     // tiles of 128 numbers K still has
                     mbar_expect_tx(bar, e_at + halves * (1 + sides) * MX_TILE_BYTES);
                     tma_load_2d(dst, &tmW, kb * (BOTH_K / 2), nt * BOTH_ROWS, bar);
-                    tma_load_2d(dst + x_at, &tmX, kb * (BOTH_K / 2), m0, bar);
+                    if (!(a.test_skip_copy && issued == 0)) tma_load_2d(dst + x_at, &tmX, kb * (BOTH_K / 2), m0, bar);
                     // (neighbouring tiles along K are neighbours in memory)
                     bulk_load(dst + e_at, a.g.sc + ((size_t)nt * tiles_k + 2 * kb) * MX_TILE_BYTES, halves * MX_TILE_BYTES, bar);
                     for (int q = 0; q < sides; q++)                  // (past the last token: any exponents, those sums are not stored)
@@ -178,6 +178,7 @@ static int launch_both(MxBoth a, const void *x, int bn, int S, cudaStream_t stre
     const int all_kb = (g.K + BOTH_K - 1) / BOTH_K, sides = bn > 128 ? 2 : 1;
     const int stage_bytes = (BOTH_A_BYTES + bn * (BOTH_K / 2) + 2 * (1 + sides) * MX_TILE_BYTES + 1023) & ~1023;
     a.bn = bn;
+    a.test_skip_copy = g_mx_test_skip_copy;
     a.stages = (BOTH_SMEM - 1024) / stage_bytes;
     if (a.stages > BOTH_MAX_STAGES) a.stages = BOTH_MAX_STAGES;
     a.kb_per_split = (all_kb + S - 1) / S;

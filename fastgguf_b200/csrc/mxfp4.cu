@@ -6,30 +6,27 @@
 // e = max(E - 2, 0) with E the exponent field of the float32 maximum.  x 2^(127 - e) is exact, and one conversion rounds it to the nearest
 // code, ties to the even one, beyond 6 to 6.  An infinity or no number anywhere in a block: e = 255, codes 0.
 //
-// A CTA takes 128 rows x 128 numbers: 16 threads a row with eight numbers each (loads of 16 bytes of bfloat16, two of 16 of float32), four
-// threads a block, whose maximum takes two shuffles.  The exponents of the tile are 512 neighbouring bytes, gathered in shared memory.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, bool vec, float (&v)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float *p, bool vec, float (&v)[8]) {
-    if (vec) {
-        const float4 a = __ldcs((const float4 *)p), b = __ldcs((const float4 *)p + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
+// A CTA takes 128 rows x 128 numbers.  A thread reads 32 bytes of a row at a time, 8 float32 or 16 bfloat16 numbers; the four or two threads of
+// a block find its maximum by shuffles.  The exponents of the tile are 512 neighbouring bytes, gathered in shared memory.
+__device__ __forceinline__ void load_piece(const float *p, bool vec, float (&v)[8]) {
+    if (vec)
+        asm("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(p));
+    else {
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = p[j];
     }
 }
-template <>
-__device__ __forceinline__ void load8<bf16>(const bf16 *p, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void load_piece(const bf16 *p, bool vec, float (&v)[16]) {
     if (vec) {
-        const uint4 a = __ldcs((const uint4 *)p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        uint32_t w[8];
+        asm("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
 #pragma unroll
-        for (int j = 0; j < 4; j++) { v[2 * j] = __uint_as_float(w[j] << 16); v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
+        for (int j = 0; j < 8; j++) { v[2 * j] = __uint_as_float(w[j] << 16); v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = __bfloat162float(p[j]);
+        for (int j = 0; j < 16; j++) v[j] = __bfloat162float(p[j]);
     }
 }
 // two numbers to a byte, the first in its low half
@@ -39,48 +36,52 @@ __device__ __forceinline__ uint32_t to_e2m1x2(float lo, float hi) {
     return r;
 }
 
-#define QUANT_ROWS 16      // rows a pass of the CTA's 256 threads takes
 template <typename T>
 __global__ void __launch_bounds__(256)
 mxfp4_quantize_kernel(const T *__restrict__ x, long long ldx, long long x_stride, uint8_t *__restrict__ data, uint8_t *__restrict__ scales, int R,
                       int K, int tiles_r, int vec) {
+    constexpr int V = 32 / sizeof(T), THREADS = 128 / V, ROWS = 256 / THREADS;      // numbers a piece, threads a row, rows a pass of the CTA
     __shared__ __align__(16) uint8_t tile[MX_TILE_BYTES];
     const int tk = blockIdx.x, tr = blockIdx.y % tiles_r, mat = blockIdx.y / tiles_r, tiles_k = gridDim.x;
-    const int c = threadIdx.x & 15, k = tk * 128 + c * 8, rows = min(128, R - tr * 128);
+    const int c = threadIdx.x % THREADS, k = tk * 128 + c * V, rows = min(128, R - tr * 128);
     if (threadIdx.x < 32) ((uint4 *)tile)[threadIdx.x] = make_uint4(0, 0, 0, 0);
     pdl_wait();
     pdl_launch_dependents();
     __syncthreads();
     const T *src = x + (size_t)mat * x_stride + k;
     uint8_t *dst = data + (size_t)mat * R * (K / 2) + k / 2;
-    // (whole warps leave the loop together unless the tile's rows end inside a warp's two: the shuffles name all lanes, so all walk it)
+    // (every thread walks all passes: the shuffles name all lanes)
 #pragma unroll 4
-    for (int r0 = 0; r0 < rows; r0 += QUANT_ROWS) {
-        const int rl = r0 + (threadIdx.x >> 4);
+    for (int r0 = 0; r0 < rows; r0 += ROWS) {
+        const int rl = r0 + threadIdx.x / THREADS;
         const bool live = rl < rows && k < K;
         const size_t r = (size_t)tr * 128 + rl;
-        float v[8];
-        if (live) load8<T>(src + r * ldx, vec, v);
+        float v[V];
+        if (live) load_piece(src + r * ldx, vec, v);
         else {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = 0.f;
+            for (int j = 0; j < V; j++) v[j] = 0.f;
         }
         uint32_t top = 0;                                  // the largest magnitude's bits: order as integers, NaN above infinity
 #pragma unroll
-        for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        for (int j = 0; j < V; j++) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < MX_BLOCK / V; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         const uint32_t E = top >> 23;
         const uint32_t e = E == 255 ? 255 : E > 2 ? E - 2 : 0;
         const float up = __uint_as_float((254 - min(e, 253u)) << 23);      // 2^(127 - e)
-        uint32_t w = 0;
-        if (E != 255) {
+        uint32_t w[V / 8];
 #pragma unroll
-            for (int j = 0; j < 4; j++) w |= to_e2m1x2(v[2 * j] * up, v[2 * j + 1] * up) << (8 * j);
+        for (int i = 0; i < V / 8; i++) {
+            w[i] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[i] |= to_e2m1x2(v[8 * i + 2 * j] * up, v[8 * i + 2 * j + 1] * up) << (8 * j);
+            if (E == 255) w[i] = 0;
         }
         if (live) {
-            *(uint32_t *)(dst + r * (K / 2)) = w;
-            if ((c & 3) == 0) tile[(rl & 31) * 16 + (rl >> 5) * 4 + (c >> 2)] = (uint8_t)e;
+            if constexpr (V == 16) *(uint2 *)(dst + r * (K / 2)) = make_uint2(w[0], w[1]);
+            else *(uint32_t *)(dst + r * (K / 2)) = w[0];
+            if (c % (MX_BLOCK / V) == 0) tile[(rl & 31) * 16 + (rl >> 5) * 4 + c / (MX_BLOCK / V)] = (uint8_t)e;
         }
     }
     __syncthreads();
@@ -96,8 +97,8 @@ extern "C" int fg_mxfp4_quantize(const void *x, int dtype, long long ldx, long l
     if (mats == 0 || R == 0) return 0;
     const int tiles_r = mx_tiles(R);
     if ((long long)tiles_r * mats > 65535) return FG_ERR_BAD_SIZE;
-    const int size = dtype == FG_F32 ? 4 : 2;
-    const int vec = ((uintptr_t)x & 15) == 0 && (ldx * size) % 16 == 0 && (x_stride * size) % 16 == 0;
+    const int V = dtype == FG_F32 ? 8 : 16;
+    const int vec = (uintptr_t)x % 32 == 0 && ldx % V == 0 && x_stride % V == 0;
     dim3 grid(mx_tiles(K), tiles_r * mats);
     if (dtype == FG_F32)
         return mx_launch(mxfp4_quantize_kernel<float>, grid, 256, 0, dim3(1, 1, 1), stream, (const float *)x, ldx, x_stride, (uint8_t *)data, (uint8_t *)scales, R, K, tiles_r, vec);
@@ -105,49 +106,67 @@ extern "C" int fg_mxfp4_quantize(const void *x, int dtype, long long ldx, long l
 }
 
 // ---------------------------------------------------------------------------- rows
-// out[i] = scale * row rows[i] (null: row i), a thread sixteen bytes of output: four float32 or eight bfloat16 numbers, which lie in one block.
-// The number itself is exact in either type; a scale other than 1 rounds once.  A row index outside the matrix gives a row of NaN.
+// out[i] = scale * row rows[i] (null: row i).  A piece is eight numbers, which lie in one block: four bytes in, 16 or 32 out.  A thread takes four
+// pieces, 256 apart, and asks for all of them before it converts the first.  The number itself is exact in either type; a scale other than 1 rounds
+// once.  A row index outside the matrix gives a row of NaN.
+#define ROWS_PIECES 4
+__device__ __forceinline__ void store8(float *p, bool vec, const float (&v)[8]) {
+    if (vec)
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) p[j] = v[j];
+    }
+}
+__device__ __forceinline__ void store8(bf16 *p, bool vec, const float (&v)[8]) {
+    if (vec) {
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) { __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]); q[j] = *(uint32_t *)&t; }
+        *(uint4 *)p = make_uint4(q[0], q[1], q[2], q[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) p[j] = __float2bfloat16_rn(v[j]);
+    }
+}
+// pieces 0 .. total - 1 of the rows from r0 on; `over` is 2^64 / (pieces a row) rounded up, by which a piece's row is one multiplication
 template <typename T>
 __global__ void __launch_bounds__(256)
 mxfp4_rows_kernel(const uint8_t *__restrict__ data, const uint8_t *__restrict__ scales, const int *__restrict__ rows, T *__restrict__ out,
-                  long long ldo, long long total, int R, int K, float scale, int vec) {
-    constexpr int V = 16 / sizeof(T);
-    const int per_row = K / V, tiles_k = mx_tiles(K);
+                  long long ldo, int r0, unsigned total, unsigned long long over, int R, int K, float scale, int vec) {
+    const int tiles_k = mx_tiles(K);
+    const unsigned at0 = blockIdx.x * (256 * ROWS_PIECES) + threadIdx.x, per_row = K / 8;
+    uint32_t w[ROWS_PIECES], e[ROWS_PIECES];
+    long long to[ROWS_PIECES];
     pdl_wait();
-    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long long)gridDim.x * 256) {
-        const long long i = at / per_row;
-        const int c = (int)(at - i * per_row) * V;
-        const int r = rows ? rows[i] : (int)i;
-        const bool ok = r >= 0 && r < R;
-        uint32_t w = 0, e = 255;
-        if (ok) {
-            const uint8_t *src = data + (size_t)r * (K / 2) + c / 2;
-            w = V == 8 ? *(const uint32_t *)src : (uint32_t) * (const uint16_t *)src;
-            e = scales[mx_scale_at(r, c / MX_BLOCK, tiles_k)];
-        }
-        const float p = mx_power(e);
-        float v[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            const uint32_t code = (w >> (4 * j)) & 15;
-            // the code's value bits as a float32's lowest exponent and highest mantissa bits are the number times 2^-126
-            v[j] = scale * (__uint_as_float((code >> 3 << 31) | ((code & 7) << 22)) * __uint_as_float(253u << 23) * p);
-        }
-        T *dst = out + (size_t)i * ldo + c;
-        if (vec) {
-            uint4 o;
-            if constexpr (V == 4) o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-            else {
-                uint32_t q[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) { __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]); q[j] = *(uint32_t *)&t; }
-                o = make_uint4(q[0], q[1], q[2], q[3]);
+    for (int p = 0; p < ROWS_PIECES; p++) {
+        const unsigned at = at0 + p * 256;
+        w[p] = 0;
+        e[p] = 255;
+        if (at < total) {
+            const unsigned i = per_row == 1 ? at : (unsigned)__umul64hi(at, over);
+            const int c = (int)(at - i * per_row) * 8, r = rows ? rows[r0 + i] : r0 + (int)i;
+            to[p] = (long long)(r0 + (int)i) * ldo + c;
+            if (r >= 0 && r < R) {
+                w[p] = *(const uint32_t *)(data + (size_t)r * (K / 2) + c / 2);
+                e[p] = scales[mx_scale_at(r, c / MX_BLOCK, tiles_k)];
             }
-            *(uint4 *)dst = o;
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; j++) dst[j] = from_f32<T>(v[j]);
         }
+    }
+#pragma unroll
+    for (int p = 0; p < ROWS_PIECES; p++) {
+        if (at0 + p * 256 >= total) break;
+        const float f = mx_power(e[p]);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t code = w[p] >> (4 * j);
+            // the code's value bits as a float32's lowest exponent and highest mantissa bits are the number times 2^-126
+            v[j] = scale * (__uint_as_float((code & 8) << 28 | (code & 7) << 22) * __uint_as_float(253u << 23) * f);
+        }
+        store8(out + to[p], vec, v);
     }
 }
 
@@ -156,12 +175,18 @@ extern "C" int fg_mxfp4_rows(const void *data, const void *scales, const int *ro
                              float scale, cudaStream_t stream) {
     if (out_dtype != FG_F32 && out_dtype != FG_BF16) return FG_ERR_BAD_DTYPE;
     if (n < 0 || R < 0 || K <= 0 || K % MX_BLOCK || ldo < K || (!rows && n > R) || ((uintptr_t)data & 3)) return FG_ERR_BAD_SIZE;
-    if (n == 0) return 0;
-    const int V = out_dtype == FG_F32 ? 4 : 8;
-    const int vec = ((uintptr_t)out & 15) == 0 && ldo % V == 0;
-    const long long total = (long long)n * (K / V), want = (total + 255) / 256;
-    dim3 grid((unsigned)(want < 148 * 64 ? want : 148 * 64));
-    if (out_dtype == FG_F32)
-        return mx_launch(mxfp4_rows_kernel<float>, grid, 256, 0, dim3(1, 1, 1), stream, (const uint8_t *)data, (const uint8_t *)scales, rows, (float *)out, ldo, total, R, K, scale, vec);
-    return mx_launch(mxfp4_rows_kernel<bf16>, grid, 256, 0, dim3(1, 1, 1), stream, (const uint8_t *)data, (const uint8_t *)scales, rows, (bf16 *)out, ldo, total, R, K, scale, vec);
+    const unsigned per_row = K / 8;
+    const int most = (int)(0x7fffffffu / per_row);                   // rows of a launch: pieces are counted in 31 bits
+    const unsigned long long over = ~0ull / per_row + 1;
+    const int vec = (uintptr_t)out % (out_dtype == FG_F32 ? 32 : 16) == 0 && ldo % 8 == 0;
+    for (int r0 = 0; r0 < n; r0 += most) {
+        const unsigned total = (unsigned)(n - r0 < most ? n - r0 : most) * per_row;
+        const dim3 grid((total + 256 * ROWS_PIECES - 1) / (256 * ROWS_PIECES));
+        const int rc = out_dtype == FG_F32
+            ? mx_launch(mxfp4_rows_kernel<float>, grid, 256, 0, dim3(1, 1, 1), stream, (const uint8_t *)data, (const uint8_t *)scales, rows, (float *)out, ldo, r0, total, over, R, K, scale, vec)
+            : mx_launch(mxfp4_rows_kernel<bf16>, grid, 256, 0, dim3(1, 1, 1), stream, (const uint8_t *)data, (const uint8_t *)scales, rows, (bf16 *)out, ldo, r0, total, over, R, K, scale, vec);
+        if (rc) return rc;
+        if (n - r0 <= most) break;                                   // (r0 + most may pass 31 bits)
+    }
+    return 0;
 }

@@ -562,3 +562,45 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for i, g in enumerate(got):
         assert all(torch.equal(p, q) for p, q in zip(g, want[i % 2]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["tiles", "tiles split", "pairs", "both"])
+def test_a_wait_that_runs_out_ends_the_kernel_and_the_next_is_correct(which):
+    """The first copy of tokens is left out and waits are shortened to about a millisecond: the kernel gives up, raises its error flag, frees its tensor
+    memory and returns."""
+    import time
+    from ctypes import c_int, c_longlong
+    m, n, k = 100, 300, 2048
+    w, numbers = _matrix(n, k, 8)
+    x = _rows(m, k, 9)
+    q, xd = ops.mxfp4_quantize(x.cuda()), x.cuda()
+
+    def call():
+        if which == "both":
+            return ops.gemm_mxfp4_both(q, w, out_dtype=torch.float32)
+        return _named(xd, w, 3 if which == "pairs" else 2, 112, 4 if which == "tiles split" else 1).clone()
+
+    error, hook = ops.lib("mx").fg_gemm_mxfp4_error, ops.lib("mx").fg_gemm_mxfp4_test_hook
+    hook.argtypes, hook.restype = [c_longlong, c_int], c_int
+    want, slack = plain.product(plain.rounded(x)[0] if which == "both" else x, numbers)
+    before = call()
+    plain.check(before, want, slack)
+    assert error() == 0
+    try:
+        assert hook(2_000_000, 1) == 0
+        t0 = time.time()
+        if which == "both":
+            call()
+        else:
+            out = torch.empty(m, n, device="cuda")
+            ops.lib("mx").fg_gemm_mxfp4_ext(xd.data_ptr(), k, w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), 0, n, 0, m, n, k, 3 if which == "pairs" else 2,
+                                            112, 4 if which == "tiles split" else 1, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert time.time() - t0 < 2.0
+        with pytest.raises(KernelError, match="wait ran out"):
+            ops.raise_on_device_error("test")
+    finally:
+        assert hook(0, 0) == 0
+    assert error() == 0
+    assert torch.equal(call(), before) and error() == 0
