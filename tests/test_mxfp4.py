@@ -416,7 +416,8 @@ def _runs(counts, before=0):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("counts,n,k", [([1], 64, 32), ([0, 1, 0, 2], 65, 96), ([3, 0, 9, 1, 0, 17, 2, 0], 200, 160), ([130, 1, 0, 257, 64], 129, 512),
-                                        ([0, 0, 0], 64, 64), ([1] * 40, 300, 2048), ([700, 0, 5], 384, 1056)])
+                                        ([0, 0, 0], 64, 64), ([1] * 40, 300, 2048), ([700, 0, 5], 384, 1056), ([0, 1, 2, 33, 0, 7, 1, 5], 260, 288),
+                                        ([40, 0, 90, 3], 700, 160), ([0] * 1500 + [3, 1] + [0] * 10, 40, 64)])
 def test_rows_grouped_by_expert(counts, n, k):
     P, X = sum(counts), len(counts)
     stack = [plain.random_matrix(n, k, _gen(100 + e)) for e in range(X)]
@@ -437,6 +438,17 @@ def test_rows_grouped_by_expert(counts, n, k):
     again = torch.full_like(out, 7.0)
     ops.gemm_mxfp4_grouped(x.cuda(), w, offsets, out=again)
     assert torch.equal(out, again)
+    odd = torch.zeros(x.shape[0], k + 1, dtype=torch.bfloat16, device="cuda")              # rows that TMA cannot address
+    odd[:, :k] = x.cuda()
+    other = torch.full_like(out, 7.0)
+    ops.gemm_mxfp4_grouped(odd[:, :k], w, offsets, out=other)
+    assert (other[:before] == 7).all() and (other[before + P:] == 7).all()
+    at = before
+    for c, (d, e) in zip(counts, stack):
+        if c:
+            want, slack = plain.product(x[at:at + c], plain.numbers(d, e))
+            plain.check(other[at:at + c], want, slack)
+        at += c
     if P:
         ops.gemm_mxfp4_grouped(x.cuda(), w, offsets, out=again, accumulate=True)
         assert torch.equal(again[before:before + P], 2 * out[before:before + P])
