@@ -99,32 +99,31 @@ class Mxfp4:
 
 
 _launchers: dict = {}
+_current_device, _raw_stream = torch.cuda.current_device, getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _launch(name: str, device: int, *args) -> None:
-    """Calls a launcher on the tensors' device, whichever is current, and that device's current stream.  (A small step's time is the host's: what a call
-    needs is looked up once.)"""
+    """Calls a launcher on the tensors' device, whichever is current, and on that device's current stream.  (A small step's time is the host's: what a
+    call needs is looked up once.)"""
     fn = _launchers.get(name)
     if fn is None:
         fn = _launchers[name] = getattr(lib("mx"), "fg_" + name)
-    if device == torch.cuda.current_device():
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device)), name)
+    if device == _current_device():
+        code = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(device)), name)
+            code = fn(*args, _raw_stream(device))
+    check(code, name)
 
 
-def _same_device(what: str, device: torch.device, *tensors) -> None:
+def _on_one_device(what: str, *tensors) -> int:
+    """The CUDA device that holds all of the tensors (None: left out)."""
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise KernelError(f"{what}: tensors on {device} and {t.device}")
-
-
-def _out_code(what: str, dtype: torch.dtype) -> int:
-    code = _CODES.get(dtype)
-    if code is None:
-        raise KernelError(f"{what}: cannot write {dtype}")
-    return code
+        if t is not None and (t.get_device() != device or device < 0):
+            require_cuda(*tensors)
+            raise KernelError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+    return device
 
 
 def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
@@ -157,7 +156,7 @@ def mxfp4_rows(w: Mxfp4, rows: Optional[torch.Tensor] = None, *, scale: float = 
                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """out[i, :] = scale * w[rows[i], :] (without ``rows``: every row), float32 or bfloat16: what the matrix stands for, or the lookup in an
     embedding table.  rows: [n] int32.  A row index outside the matrix gives a row of NaN."""
-    require_cuda(w.data, rows, out)
+    device = _on_one_device("mxfp4_rows", w.data, rows, out)
     if w.data.dim() != 2:
         raise KernelError("mxfp4_rows: w is one matrix, not a stack")
     if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous()):
@@ -167,9 +166,10 @@ def mxfp4_rows(w: Mxfp4, rows: Optional[torch.Tensor] = None, *, scale: float = 
         out = w.data.new_empty((n, w.k), dtype=out_dtype or torch.float32)
     elif out.shape != (n, w.k) or out.stride(1) != 1 or (n > 1 and out.stride(0) < w.k) or (out_dtype is not None and out.dtype != out_dtype):
         raise KernelError(f"mxfp4_rows: out must be [{n}, {w.k}] with contiguous rows")
-    code = _out_code("mxfp4_rows", out.dtype)
-    _same_device("mxfp4_rows", w.device, rows, out)
-    _launch("mxfp4_rows", out.get_device(), w.data.data_ptr(), w.scales.data_ptr(), rows.data_ptr() if rows is not None else None, out.data_ptr(), code,
+    code = _CODES.get(out.dtype)
+    if code is None:
+        raise KernelError(f"mxfp4_rows: cannot write {out.dtype}")
+    _launch("mxfp4_rows", device, w.data.data_ptr(), w.scales.data_ptr(), rows.data_ptr() if rows is not None else None, out.data_ptr(), code,
             max(out.stride(0), w.k), n, w.rows, w.k, scale)
     return out
 
@@ -181,7 +181,9 @@ def _output(what: str, M: int, N: int, like: torch.Tensor, out, out_dtype, accum
         out = like.new_empty((M, N), dtype=out_dtype or torch.bfloat16)
     elif out.shape != (M, N) or out.stride(1) != 1 or (M > 1 and out.stride(0) < N) or (out_dtype is not None and out.dtype != out_dtype):
         raise KernelError(f"{what}: out must be [{M}, {N}] with contiguous rows")
-    code = _out_code(what, out.dtype)
+    code = _CODES.get(out.dtype)
+    if code is None:
+        raise KernelError(f"{what}: cannot write {out.dtype}")
     if accumulate and code != FG_F32:
         raise KernelError(f"{what}: the residual sum is 32-bit; accumulate needs a float32 output")
     return out, code
@@ -200,14 +202,14 @@ def gemm_mxfp4(x: torch.Tensor, w: Mxfp4, *, out: Optional[torch.Tensor] = None,
                accumulate: bool = False) -> torch.Tensor:
     """out[m, n] (+)= sum_k x[m, k] w[n, k]: bfloat16 activations [M, K] on a matrix [N, K] in MXFP4, float32 sums.  Output bfloat16 (default) or
     float32; ``accumulate`` adds into a float32 ``out``."""
-    require_cuda(x, w.data, out)
-    if w.data.dim() != 2:
+    data = w.data
+    device = _on_one_device("gemm_mxfp4", x, data, out)
+    if data.dim() != 2:
         raise KernelError("gemm_mxfp4: w is one matrix, not a stack (see gemm_mxfp4_grouped)")
     _activations("gemm_mxfp4", x, w.k)
     M = x.shape[0]
-    out, code = _output("gemm_mxfp4", M, w.rows, w.data, out, out_dtype, accumulate)
-    _same_device("gemm_mxfp4", x.device, w.data, out)
-    _launch("gemm_mxfp4", x.get_device(), x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, out.stride(0),
+    out, code = _output("gemm_mxfp4", M, w.rows, data, out, out_dtype, accumulate)
+    _launch("gemm_mxfp4", device, x.data_ptr(), x.stride(0), data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, out.stride(0),
             accumulate, M, w.rows, w.k)
     return out
 
@@ -215,15 +217,14 @@ def gemm_mxfp4(x: torch.Tensor, w: Mxfp4, *, out: Optional[torch.Tensor] = None,
 def gemm_mxfp4_both(x: Mxfp4, w: Mxfp4, *, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
                     accumulate: bool = False) -> torch.Tensor:
     """The same with the activations [M, K] in MXFP4 too (``mxfp4_quantize``)."""
-    require_cuda(x.data, w.data, out)
+    device = _on_one_device("gemm_mxfp4_both", x.data, w.data, out)
     if w.data.dim() != 2 or x.data.dim() != 2:
         raise KernelError("gemm_mxfp4_both: x and w are one matrix each, not stacks")
     if x.k != w.k:
         raise KernelError(f"gemm_mxfp4_both: x is {x.shape} but w is {w.shape}")
     M = x.rows
     out, code = _output("gemm_mxfp4_both", M, w.rows, w.data, out, out_dtype, accumulate)
-    _same_device("gemm_mxfp4_both", x.device, w.data, out)
-    _launch("gemm_mxfp4_both", out.get_device(), x.data.data_ptr(), x.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code,
+    _launch("gemm_mxfp4_both", device, x.data.data_ptr(), x.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code,
             out.stride(0), accumulate, M, w.rows, w.k)
     return out
 
@@ -234,7 +235,7 @@ def gemm_mxfp4_grouped(x: torch.Tensor, w: Mxfp4, offsets: torch.Tensor, *, out:
 
     x: [M, K] bfloat16; w: a stack [X, N, K]; offsets: [X + 1] int32 on the device, rising from the first row.  Runs may be empty.  Rows of no
     run (before the first offset, behind the last) are not written: they keep what ``out`` held, which is undefined without an ``out``."""
-    require_cuda(x, w.data, offsets, out)
+    device = _on_one_device("gemm_mxfp4_grouped", x, w.data, offsets, out)
     if w.data.dim() != 3:
         raise KernelError("gemm_mxfp4_grouped: w is a stack of matrices")
     X = w.data.shape[0]
@@ -243,7 +244,6 @@ def gemm_mxfp4_grouped(x: torch.Tensor, w: Mxfp4, offsets: torch.Tensor, *, out:
     _activations("gemm_mxfp4_grouped", x, w.k)
     M = x.shape[0]
     out, code = _output("gemm_mxfp4_grouped", M, w.rows, w.data, out, out_dtype, accumulate)
-    _same_device("gemm_mxfp4_grouped", x.device, w.data, offsets, out)
-    _launch("gemm_mxfp4_grouped", x.get_device(), x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), offsets.data_ptr(), X, out.data_ptr(),
+    _launch("gemm_mxfp4_grouped", device, x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), offsets.data_ptr(), X, out.data_ptr(),
             code, out.stride(0), accumulate, M, w.rows, w.k)
     return out

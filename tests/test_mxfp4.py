@@ -71,10 +71,20 @@ def test_there_is_no_cpu_path():
             call()
 
 
+@pytest.mark.gpu
+def test_tensors_on_two_devices_are_refused():
+    w, _ = _matrix(4, 64, 1)
+    here = torch.zeros(2, 64, dtype=torch.bfloat16)
+    for call in (lambda: ops.gemm_mxfp4(here, w), lambda: ops.gemm_mxfp4(here.cuda(), w, out=torch.zeros(2, 4)), lambda: ops.mxfp4_rows(w, torch.zeros(1, dtype=torch.int32))):
+        with pytest.raises(KernelError, match="cpu"):
+            call()
+
+
 @pytest.fixture
 def no_device_check(monkeypatch):
     from fastgguf_b200.ops import mxfp4
     monkeypatch.setattr(mxfp4, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(mxfp4, "_on_one_device", lambda *t: 0)
     monkeypatch.setattr(mxfp4, "_launch", lambda *a: pytest.fail("a refused call reached a kernel"))
 
 
