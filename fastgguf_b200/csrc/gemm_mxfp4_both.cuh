@@ -97,19 +97,30 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                 ok = mbar_wait_warp(full0 + 8 * s, ph);
                 if (!ok) { mx_raise(2); break; }
                 tc_fence_after();
+                const uint32_t base16 = (smem0 + s * stage_bytes) >> 4, e16 = base16 + (e_at >> 4), ad = base16 | 1u << 16, bd = ad + (x_at >> 4);
+                // exponents of this stage: columns 256 + 24 s: weights [half][4], tokens [half][side][4]
+                const uint32_t ea = tmem + 256 + s * 24, eb = ea + 8;
+                const int left = a.g.K - (kb0 + kb) * BOTH_K;
                 if (elect_one()) {
-                    const uint32_t base = smem0 + s * stage_bytes;
-                    const int left = a.g.K - (kb0 + kb) * BOTH_K, steps = min(4, (left + 63) / 64), halves = min(2, (left + 127) / 128);
-                    // exponents of this stage: columns 256 + 24 s: weights [half][4], tokens [half][side][4]
-                    const uint32_t ea = tmem + 256 + s * 24, eb = ea + 8;
-                    for (int h = 0; h < halves; h++) {
-                        tc_cp_exponents(ea + 4 * h, base + e_at + h * MX_TILE_BYTES);
-                        for (int q = 0; q < sides; q++) tc_cp_exponents(eb + 8 * h + 4 * q, base + e_at + (2 + 2 * q + h) * MX_TILE_BYTES);
-                    }
-                    const uint64_t ad = mx_smem_desc(base), bd = mx_smem_desc(base + x_at);
-                    for (int k = 0; k < steps; k++) {
-                        const uint32_t id = (k & 1) * 2;
-                        tc_mma_mxf4(tmem, ad + 2 * k, bd + 2 * k, idesc | id << 4 | id << 29, ea + 4 * (k >> 1), eb + 8 * (k >> 1), (kb | k) != 0);
+                    // (a whole stage as straight code: a step's operands cost more cycles than the step where they are computed one by one)
+                    if (left >= BOTH_K) {
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            tc_cp_exponents(ea + 4 * h, e16 + h * (MX_TILE_BYTES >> 4));
+                            tc_cp_exponents(eb + 8 * h, e16 + (2 + h) * (MX_TILE_BYTES >> 4));
+                            if (sides == 2) tc_cp_exponents(eb + 8 * h + 4, e16 + (4 + h) * (MX_TILE_BYTES >> 4));
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            tc_mma_mxf4(tmem, ad + 2 * k, bd + 2 * k, idesc | (k & 1) * (2u << 4 | 2u << 29), ea + 4 * (k >> 1), eb + 8 * (k >> 1), (kb | k) != 0);
+                    } else {
+                        const int steps = (left + 63) / 64, halves = (left + 127) / 128;
+                        for (int h = 0; h < halves; h++) {
+                            tc_cp_exponents(ea + 4 * h, e16 + h * (MX_TILE_BYTES >> 4));
+                            for (int q = 0; q < sides; q++) tc_cp_exponents(eb + 8 * h + 4 * q, e16 + (2 + 2 * q + h) * (MX_TILE_BYTES >> 4));
+                        }
+                        for (int k = 0; k < steps; k++)
+                            tc_mma_mxf4(tmem, ad + 2 * k, bd + 2 * k, idesc | (k & 1) * (2u << 4 | 2u << 29), ea + 4 * (k >> 1), eb + 8 * (k >> 1), (kb | k) != 0);
                     }
                     tc_commit(empty0 + 8 * s);
                 }

@@ -109,17 +109,22 @@ __device__ __forceinline__ void tc_mma_bf16_ts_pair(uint32_t d, uint32_t a, uint
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(acc) : "memory");
 }
+// Operands in shared memory: K-major tiles, rows of 128 bytes swizzled by 128, 8-row groups 1024 bytes apart.  Of the descriptor only the lower word (mx_desc_lo)
+// changes between MMAs, by the address in units of 16 bytes; the upper one is a constant.
+#define MX_DESC_HI 0x40004040
+__device__ __forceinline__ uint32_t mx_desc_lo(uint32_t saddr) { return (saddr & 0x3FFFF) >> 4 | 1u << 16; }
 // D (tensor memory) (+)= A B^T of 4-bit numbers whose blocks of 32 share a power of two, 64 numbers of K; both operands in shared memory, the
 // exponents in tensor memory
-__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t ea, uint32_t eb, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(ea), "r"(eb), "r"(acc) : "memory");
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t ea, uint32_t eb, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %6, 0;\n\tmov.b64 a, {%1, %7};\n\tmov.b64 b, {%2, %7};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n\t}"
+                 ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(ea), "r"(eb), "r"(acc), "n"(MX_DESC_HI) : "memory");
 }
-// 512 bytes of exponents (32 rows of 16) from shared memory to four columns of tensor memory, the same for each group of 32 lanes
-__device__ __forceinline__ void tc_cp_exponents(uint32_t taddr, uint32_t saddr) {
-    const uint64_t desc = (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;      // 8 rows every 128 bytes, not swizzled
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+// 512 bytes of exponents (32 rows of 16: 8 rows every 128 bytes, not swizzled) from shared memory to four columns of tensor memory, the same for each
+// group of 32 lanes; the address in units of 16 bytes
+__device__ __forceinline__ void tc_cp_exponents(uint32_t taddr, uint32_t saddr16) {
+    asm volatile("{\n\t.reg .b64 s;\n\tmov.b64 s, {%1, %2};\n\t"
+                 "tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], s;\n\t}" ::"r"(taddr), "r"(saddr16), "n"(0x4008) : "memory");
 }
 // sixteen columns of this lane's row, without the wait
 __device__ __forceinline__ void tc_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
