@@ -455,7 +455,7 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (a pair's leader alone)
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)((PAIR ? 2 : 1) * TILE_ROWS >> 4) << 24);
-        const uint64_t desc0 = mx_smem_desc(smem0);
+        const uint32_t desc0 = mx_desc_lo(smem0);
         int g = 0, s = 0, i = 0;
         bool ok = rank == 0;
         for (int T = first; T < n_tiles && ok; T += stride, i++) {
@@ -466,14 +466,13 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                 ok = mbar_wait_warp(full0 + 8 * slot, (g / TILE_SLOTS) & 1);
                 if (!ok) { mx_raise(2); break; }
                 tc_fence_after();
-                const uint64_t desc = desc0 + (uint64_t)(s * (x_bytes >> 4));
+                const uint32_t desc[2] = {desc0 + s * (x_bytes >> 4), desc0 + s * (x_bytes >> 4) + (x_half >> 4)};
                 const uint32_t at = tmem + 256 + slot * 64;
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
-                        const uint64_t d = desc + (uint64_t)((k >> 2) * (x_half >> 4) + (k & 3) * 2);
-                        if (PAIR) tc_mma_bf16_ts_pair(tmem, at + k * 8, d, idesc, (kb | k) != 0);
-                        else tc_mma_bf16_ts(tmem, at + k * 8, d, idesc, (kb | k) != 0);
+                        if (PAIR) tc_mma_bf16_ts_pair(tmem, at + k * 8, desc[k >> 2] + (k & 3) * 2, idesc, (kb | k) != 0);
+                        else tc_mma_bf16_ts(tmem, at + k * 8, desc[k >> 2] + (k & 3) * 2, idesc, (kb | k) != 0);
                     }
                     if (PAIR) tc_commit_pair(done0 + 8 * slot); else tc_commit(done0 + 8 * slot);
                 }

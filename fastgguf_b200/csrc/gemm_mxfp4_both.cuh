@@ -97,7 +97,7 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
                 ok = mbar_wait_warp(full0 + 8 * s, ph);
                 if (!ok) { mx_raise(2); break; }
                 tc_fence_after();
-                const uint32_t base16 = (smem0 + s * stage_bytes) >> 4, e16 = base16 + (e_at >> 4), ad = base16 | 1u << 16, bd = ad + (x_at >> 4);
+                const uint32_t base16 = (smem0 + s * stage_bytes) >> 4, e16 = base16 + (e_at >> 4), ad = mx_desc_lo(smem0 + s * stage_bytes), bd = ad + (x_at >> 4);
                 // exponents of this stage: columns 256 + 24 s: weights [half][4], tokens [half][side][4]
                 const uint32_t ea = tmem + 256 + s * 24, eb = ea + 8;
                 const int left = a.g.K - (kb0 + kb) * BOTH_K;

@@ -97,22 +97,22 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
 __device__ __forceinline__ void tc_free(uint32_t base, uint32_t columns) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
 }
-// D (tensor memory) (+)= A B^T in bfloat16, A in tensor memory (a lane a row, two neighbouring k a column), B in shared memory
-__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(acc) : "memory");
-}
-// the same with A and D spread over the tensor memory of a pair of CTAs, B over their shared memory
-__device__ __forceinline__ void tc_mma_bf16_ts_pair(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(acc) : "memory");
-}
 // Operands in shared memory: K-major tiles, rows of 128 bytes swizzled by 128, 8-row groups 1024 bytes apart.  Of the descriptor only the lower word (mx_desc_lo)
 // changes between MMAs, by the address in units of 16 bytes; the upper one is a constant.
 #define MX_DESC_HI 0x40004040
 __device__ __forceinline__ uint32_t mx_desc_lo(uint32_t saddr) { return (saddr & 0x3FFFF) >> 4 | 1u << 16; }
+// D (tensor memory) (+)= A B^T in bfloat16, A in tensor memory (a lane a row, two neighbouring k a column), B in shared memory
+__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(acc), "n"(MX_DESC_HI) : "memory");
+}
+// the same with A and D spread over the tensor memory of a pair of CTAs, B over their shared memory
+__device__ __forceinline__ void tc_mma_bf16_ts_pair(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(acc), "n"(MX_DESC_HI) : "memory");
+}
 // D (tensor memory) (+)= A B^T of 4-bit numbers whose blocks of 32 share a power of two, 64 numbers of K; both operands in shared memory, the
 // exponents in tensor memory
 __device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t ea, uint32_t eb, uint32_t acc) {
@@ -142,10 +142,6 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&w)[16])
                    "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15]) : "memory");
 }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// K-major tile, rows of 128 bytes swizzled by 128, 8-row groups 1024 bytes apart
-__device__ __forceinline__ uint64_t mx_smem_desc(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
 __device__ __forceinline__ void cluster_sync_all() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
