@@ -3,6 +3,7 @@
     python -m fastgguf_b200.kernel_bench attention_prefill [--head-dim 64] [--heads 32] [--kv-heads 8]
     python -m fastgguf_b200.kernel_bench attention_decode  [--head-dim 64] [--heads 32] [--kv-heads 8]
     python -m fastgguf_b200.kernel_bench gemm [--hidden 2048] [--qkv 3072] [--ffn 8192]
+    python -m fastgguf_b200.kernel_bench mxfp4 [--hidden 2048] [--ffn 8192] [--experts 32]
     python -m fastgguf_b200.kernel_bench prompt_steps [--hidden 2048 --layers 16 --heads 32 --kv-heads 8 --head-dim 64
                                                        --ffn 8192 --vocab 128256]
 
@@ -20,6 +21,7 @@ import os
 
 import torch
 
+from . import ops
 from .ops import fast_attention, fast_gemm
 
 PAGE = 64
@@ -135,6 +137,33 @@ def gemm(args):
         raise RuntimeError("a bounded wait of a contraction ran out")
 
 
+def mxfp4(args):
+    """Matrices in microscaled 4-bit floating point over row counts: gate and up of a feed-forward with bfloat16 and with quantised activations, the
+    quantiser, and experts of hidden x hidden with two a token."""
+    hbm, tf = _peaks()
+    E, N, X = args.hidden, 2 * args.ffn, args.experts
+    time = _Timer(flush=True)
+    w = ops.mxfp4_quantize(torch.randn(N, E, device="cuda") * E ** -0.5)
+    stack = ops.mxfp4_quantize(torch.randn(X, E, E, device="cuda") * E ** -0.5)
+    for M in (1, 8, 16, 64, 128, 256, 512, 1024, 2048, 4096):
+        x = torch.randn(M, E, device="cuda", dtype=torch.bfloat16)
+        q, out = ops.mxfp4_quantize(x), torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+        pairs = torch.randn(2 * M, E, device="cuda", dtype=torch.bfloat16)
+        expert = torch.randint(0, X, (2 * M,), device="cuda")
+        offsets = torch.cat([torch.zeros(1, dtype=torch.int64, device="cuda"), torch.bincount(expert, minlength=X).cumsum(0)]).to(torch.int32)
+        expert_out = torch.empty_like(pairs)
+        cells = []
+        for label, fn, nbytes, flops in [
+                ("bfloat16 x 4-bit", lambda: ops.gemm_mxfp4(x, w, out=out), N * E * 17 / 32 + 2 * M * (E + N), 2.0 * M * N * E),
+                ("4-bit x 4-bit", lambda: ops.gemm_mxfp4_both(q, w, out=out), (N + M) * E * 17 / 32 + 2 * M * N, 2.0 * M * N * E),
+                ("quantise", lambda: ops.mxfp4_quantize(x), M * E * (2 + 17 / 32), 0.0),
+                ("experts", lambda: ops.gemm_mxfp4_grouped(pairs, stack, offsets, out=expert_out), min(2 * M, X) * E * E * 17 / 32 + 8 * M * E, 4.0 * M * E * E)]:
+            us = time(fn)
+            cells.append(f"{label} {us:7.1f} us {nbytes / us / 1e3:5.0f} GB/s ({nbytes / us / 1e3 / hbm:4.2f})" + (f" {flops / us / 1e6:6.1f} TFLOP/s ({flops / us / 1e6 / tf:4.2f})" if flops else ""))
+        print(f"mxfp4 rows {M:5d}: " + " | ".join(cells), flush=True)
+    ops.raise_on_device_error("mxfp4")
+
+
 def prompt_steps(args):
     """Time to the first token's logits over prompt lengths: one sequence, one step, its slot given back after it."""
     import numpy as np
@@ -177,6 +206,10 @@ def main(argv=None):
     p.add_argument("--hidden", type=int, default=2048)
     p.add_argument("--qkv", type=int, default=3072)
     p.add_argument("--ffn", type=int, default=8192)
+    p = sub.add_parser("mxfp4")
+    p.add_argument("--hidden", type=int, default=2048)
+    p.add_argument("--ffn", type=int, default=8192)
+    p.add_argument("--experts", type=int, default=32)
     p = sub.add_parser("prompt_steps")
     for name, default in (("hidden", 2048), ("layers", 16), ("heads", 32), ("kv-heads", 8), ("head-dim", 64), ("ffn", 8192),
                           ("vocab", 128256)):
@@ -184,7 +217,7 @@ def main(argv=None):
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():
         raise SystemExit("kernel_bench needs a GPU")
-    {"attention_prefill": attention_prefill, "attention_decode": attention_decode, "gemm": gemm,
+    {"attention_prefill": attention_prefill, "attention_decode": attention_decode, "gemm": gemm, "mxfp4": mxfp4,
      "prompt_steps": prompt_steps}[args.what](args)
 
 

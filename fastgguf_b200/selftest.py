@@ -111,6 +111,38 @@ def run_selftest(quick: bool = False) -> int:
     r.check("gemm_tc deferred RMSNorm (started in one epilogue, finished in the next)", _rel(got, want), 2 ** -7)
     r.check("gemm_tc pipeline error flag", float(fast_gemm.pipeline_error()), 0.0)
 
+    # ---- matrices in microscaled 4-bit floating point: the numbers a quantised matrix stands for, decoded here code by code
+    def numbers(q):
+        code = torch.stack([q.data & 15, q.data >> 4], -1).reshape(q.rows, -1, 32).long()
+        size = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64, device=dev)[code & 7]
+        power = ((q.exponents().long() + (1023 - 127)) << 52).view(torch.float64)
+        return (torch.where(code >= 8, -size, size) * power[..., None]).reshape(q.rows, q.k)
+
+    x = (torch.randn(70, 352, generator=g) * torch.exp(2 * torch.randn(70, 1, generator=g))).to(dev)
+    q = ops.mxfp4_quantize(x)
+    blocks = x.double().reshape(70, -1, 32)
+    step = torch.exp2(torch.floor(torch.log2(blocks.abs().amax(-1, keepdim=True))))      # of a block's largest number's binade
+    r.check("mxfp4_quantize: distance, in the block's highest binade's size", float(((numbers(q).reshape_as(blocks) - blocks).abs() / step).max()), 0.5)
+    r.check("mxfp4_rows f32", float((ops.mxfp4_rows(q).double() - numbers(q)).abs().max()), 0.0)
+    pick = torch.randint(0, 70, (9,), generator=g, dtype=torch.int32).to(dev)
+    r.check("mxfp4_rows, picked rows in bf16", float((ops.mxfp4_rows(q, pick, out_dtype=torch.bfloat16).double() - numbers(q)[pick.long()]).abs().max()), 0.0)
+    for (M, N, K) in [(1, 256, 2048), (7, 200, 1056), (40, 300, 352), (300, 1000, 544)] + ([] if quick else [(2048, 2048, 2048)]):
+        a = (torch.randn(M, K, generator=g) * 0.5).bfloat16().to(dev)
+        w4 = ops.mxfp4_quantize((torch.randn(N, K, generator=g) * 0.5).to(dev))
+        for name, xd, got in (("gemm_mxfp4", a.double(), ops.gemm_mxfp4(a, w4, out_dtype=torch.float32)),
+                              ("gemm_mxfp4_both", numbers(ops.mxfp4_quantize(a)), ops.gemm_mxfp4_both(ops.mxfp4_quantize(a), w4, out_dtype=torch.float32))):
+            want = xd @ numbers(w4).T
+            bound = float((xd.abs() @ numbers(w4).abs().T).max())
+            r.check(f"{name} f32 out {M}x{N}x{K}", float((got.double() - want).abs().max()) / bound, 2e-6)
+    counts = [0, 5, 1, 0, 70, 3]
+    rows4 = (torch.randn(sum(counts), 352, generator=g) * 0.5).bfloat16().to(dev)
+    stack = ops.mxfp4_quantize((torch.randn(len(counts), 200, 352, generator=g) * 0.5).to(dev))
+    cuts = torch.tensor([sum(counts[:i]) for i in range(len(counts) + 1)], dtype=torch.int32)
+    got = ops.gemm_mxfp4_grouped(rows4, stack, cuts.to(dev), out_dtype=torch.float32)
+    want = torch.cat([rows4[cuts[e]:cuts[e + 1]].double() @ numbers(stack[e]).T for e in range(len(counts))])
+    r.check("gemm_mxfp4_grouped f32 out", _rel(got, want), 2e-6)
+    r.check("mxfp4 error flag", float(ops.lib("mx").fg_gemm_mxfp4_error()), 0.0)
+
     # ---- row-wise kernels
     x = (torch.randn(9, 300, generator=g) * 3).to(dev)
     w = (1 + 0.1 * torch.randn(300, generator=g)).to(dev)
