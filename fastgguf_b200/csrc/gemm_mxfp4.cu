@@ -415,8 +415,9 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
             int upto = (end - begin + bn - 1) / bn;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
-            if (e0 + lane < a.g.experts) cum[e0 + lane + 1] = sum + upto;
-            sum += __shfl_sync(0xffffffffu, upto, 31);
+            // (no more than rising offsets can make, which is what the host's check of the count covers)
+            if (e0 + lane < a.g.experts) cum[e0 + lane + 1] = min(sum + upto, a.tiles_m + a.g.experts);
+            sum = min(sum + __shfl_sync(0xffffffffu, upto, 31), a.tiles_m + a.g.experts);
         }
         if (lane == 0) cum[0] = 0;
     }

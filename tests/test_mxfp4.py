@@ -477,6 +477,23 @@ def test_offsets_that_name_no_rows_reach_none(offsets):
     assert (room[:2] == 7).all() and (room[M + 2:] == 7).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [9, 300, 1500])
+def test_runs_that_overlap_many_times_reach_nothing_else(M):
+    """Offsets that fall and rise again name every row by every other expert, far more tiles than rising offsets can: nothing outside out is written."""
+    n, k, X = 70, 64, 64
+    d, e = plain.random_matrix(n, k, _gen(210))
+    w = Mxfp4.from_exponents(d.expand(X, *d.shape).cuda(), e.expand(X, *e.shape).cuda())
+    x = _rows(M, k, 52)
+    room = torch.full((M + 4, n), 7.0, device="cuda")
+    offsets = torch.tensor([0, M] * (X // 2) + [0], dtype=torch.int32, device="cuda")
+    ops.gemm_mxfp4_grouped(x.cuda(), w, offsets, out=room[2:M + 2])
+    ops.raise_on_device_error("overlapping runs")
+    assert (room[:2] == 7).all() and (room[M + 2:] == 7).all()
+    want, slack = plain.product(x, plain.numbers(d, e))               # the matrices are alike: whoever wrote a row wrote this
+    plain.check(room[2:M + 2], want, slack)
+
+
 # ------------------------------------------------------------------------------ as a program uses them
 @pytest.mark.gpu
 def test_no_rows():
