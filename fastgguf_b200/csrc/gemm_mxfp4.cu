@@ -666,10 +666,13 @@ static void tile_plan(int M, int N, int K, bool &pair, int &bn, int &S) {
     }
 }
 
+#define MX_MOST_ROWS (0x7fffffff - 512)
 static int mx_check(const MxGemm &a) {
     if (a.out_dtype != FG_F32 && a.out_dtype != FG_BF16) return FG_ERR_BAD_DTYPE;
     if (a.accumulate && a.out_dtype != FG_F32) return FG_ERR_BAD_DTYPE;
     if (a.M < 0 || a.N <= 0 || a.K <= 0 || a.K % MX_BLOCK || a.ldx < 0 || a.ldo < 0 || ((uintptr_t)a.w & 15) || ((uintptr_t)a.sc & 15)) return FG_ERR_BAD_SIZE;
+    // rows of x and of all matrices are counted in 31 bits, up to the end of the last tile
+    if (a.M > MX_MOST_ROWS || (long long)a.N * (a.offsets ? a.experts : 1) > MX_MOST_ROWS) return FG_ERR_BAD_SIZE;
     return 0;
 }
 
@@ -704,9 +707,9 @@ extern "C" int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const 
 extern "C" int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w, const void *scales, const int *offsets, int experts, void *out,
                                      int out_dtype, long long ldo, int accumulate, int M, int N, int K, cudaStream_t stream) {
     MxGemm a = {(const bf16 *)x, (const uint8_t *)w, (const uint8_t *)scales, out, ldx, ldo, M, N, K, out_dtype, accumulate, 0, offsets, experts, 0};
+    if (experts <= 0 || experts > 65535 || !offsets) return FG_ERR_BAD_SIZE;
     const int bad = mx_check(a);
     if (bad) return bad;
-    if (experts <= 0 || experts > 65535 || !offsets) return FG_ERR_BAD_SIZE;
     if (M == 0) return 0;
     a.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     if (experts <= TILE_MAX_EXPERTS && tile_ok(a)) {

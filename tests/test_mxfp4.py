@@ -127,6 +127,20 @@ def test_calls_that_do_not_fit_are_refused_before_a_launch(no_device_check):
             call()
 
 
+def test_launchers_refuse_rows_beyond_31_bits(no_device_check):
+    """Before they touch the device or the memory (the addresses here are none)."""
+    from ctypes import c_void_p
+    L, refused, most, at = ops.lib("mx"), 10002, 2 ** 31 - 1, c_void_p(1 << 20)          # (FG_ERR_BAD_SIZE)
+    sizes = [(most, 64), (most - 500, 64), (4, most), (4, most - 500)]
+    for M, N in sizes:
+        assert L.fg_gemm_mxfp4(at, 32, at, at, at, 1, N, 0, M, N, 32, None) == refused
+        for form in (1, 2, 3):
+            assert L.fg_gemm_mxfp4_ext(at, 32, at, at, at, 1, N, 0, M, N, 32, form, 16, 1, None) == refused
+        assert L.fg_gemm_mxfp4_both(at, at, at, at, at, 1, N, 0, M, N, 32, None) == refused
+        assert L.fg_gemm_mxfp4_grouped(at, 32, at, at, at, 2, at, 1, N, 0, M, N, 32, None) == refused
+    assert L.fg_gemm_mxfp4_grouped(at, 32, at, at, at, 1000, at, 1, 3000000, 0, 4, 3000000, 32, None) == refused       # 3 10^9 rows of all experts
+
+
 # ------------------------------------------------------------------------------ quantising and reading rows
 def _border_rows():
     """Rows whose blocks hold the borders between codes and their neighbours, under maxima that set the exponent."""
