@@ -1,4 +1,4 @@
-/* The C interface of the kernel libraries (libfg_core.so, libfg_tc.so, libfg_attn.so).
+/* The C interface of the kernel libraries (libfg_core.so, libfg_tc.so, libfg_attn.so, libfg_mix.so, libfg_mx.so).
  *
  * Every function launches on `stream` and returns 0, a cudaError_t, or one of the FG_ERR_* codes
  * below; none allocates device memory.  Pointers are device pointers unless said otherwise.

@@ -40,7 +40,8 @@ __device__ __forceinline__ void mx_store(const MxGemm &a, int m, int n, float v)
 // on an SM, with no registers held for them), so the ring needs no barrier.
 //
 // What bounds it: instructions.  At the memory's rate an SM gets a chunk's 2,176 bytes of 32 rows every 92 cycles, in which its four
-// schedulers issue 368; unpacking them takes 192, the MMAs, loads and addresses some 70.
+// schedulers issue 368; unpacking them takes 192, the MMAs, loads and addresses some 70.  Measured, 8 x 28,672 x 4,096: 23.5 us (2.7 TB/s); the schedulers
+// issue in 54 % of active cycles, DRAM is at 29 %: sixteen warps do not hide all of their waits, and 896 units on 296 groups are four rounds for 3.03.
 //
 // A CTA is two groups of eight warps; a group takes a unit of 32 rows at a time, its warps a chunk each in turn.  x is staged once for all the
 // units of a CTA (in parts, for each unit again, where K is longer than the room).  The eight sums are added in shared memory, those of a cluster's
@@ -282,7 +283,10 @@ static int launch_stream(MxGemm a, int y, int busy /* of the y, that have rows *
 //   warps 3-18  four sets of four, a set to a slot: unpack every fourth stage, and at a tile's end a quarter of its epilogue.  The first
 //               stages of the next tile are unpacked BEFORE a tile's epilogue: the tensor core goes on meanwhile.
 // Unpacking is bound by the integer pipe when enough warps hide the waits around it: with two warps a scheduler, half a stage each, a
-// stage's took 1,500 cycles beside the 1,024 of its MMAs at 256 tokens (2,048 x 8,192 x 4,096: 133 us; with four: 94).
+// stage's took 1,500 cycles beside the 1,024 of its MMAs at 256 tokens (2,048 x 8,192 x 4,096: 133 us; with four: 94).  At few tokens a stage
+// takes some 650 cycles: unpacking and the chain from a free slot to the next full one, beside MMAs of 46 cycles each.
+// Measured: 77 x 8,191 x 2,080 9.5 us; 256 x 8,192 x 4,096 17.4 us (988 TFLOP/s); 2,048 x 14,336 x 4,096 158 us (1,519 TFLOP/s) in a short run, 181 at the
+// power limit; at 2,048 x 28,672 x 4,096 the tensor pipe is busy in 86 % of active cycles.
 //
 // One CTA an SM walks the tiles.  PAIR: two CTAs of a cluster take 256 weight rows x BN tokens (tcgen05.mma.cta_group::2); each unpacks its
 // own 128 rows and brings half of the tokens, which halves the bytes an SM receives per MMA.  With few tiles a cluster of single CTAs splits
