@@ -40,16 +40,16 @@ __device__ __forceinline__ void mx_store(const MxGemm &a, int m, int n, float v)
 // on an SM, with no registers held for them), so the ring needs no barrier.
 //
 // What bounds it: instructions.  At the memory's rate an SM gets a chunk's 2,176 bytes of 32 rows every 92 cycles, in which its four
-// schedulers issue 368; unpacking them takes 192, the MMAs, loads and addresses some 70.  Measured, 8 x 28,672 x 4,096: 23.5 us (2.7 TB/s); the schedulers
-// issue in 54 % of active cycles, DRAM is at 29 %: sixteen warps do not hide all of their waits, and 896 units on 296 groups are four rounds for 3.03.
+// schedulers issue 368; unpacking them takes 192, the MMAs, loads and addresses some 70.  Measured: 8 x 28,672 x 4,096 22.6 us (2.8 TB/s), one row of
+// 128,256 x 2,048 35.1 (4.0).  Sixteen warps do not hide all of their waits: with two groups of eight (23.5 us) the schedulers issued in 54 % of active
+// cycles, DRAM was at 29 %.
 //
-// A CTA is two groups of eight warps; a group takes a unit of 32 rows at a time, its warps a chunk each in turn.  x is staged once for all the
-// units of a CTA (in parts, for each unit again, where K is longer than the room).  The eight sums are added in shared memory, those of a cluster's
+// A CTA is two groups of eight warps or four of four; a group takes a unit of 32 rows at a time, its warps a chunk each in turn.  x is staged once for all the
+// units of a CTA (in parts, for each unit again, where K is longer than the room).  The warps' sums are added in shared memory, those of a cluster's
 // CTAs (a split of K where there are few units, or K is long) through distributed shared memory, all in a fixed order.
 #define STREAM_ROWS 32
-#define STREAM_WARPS 8                      // of a group
-#define STREAM_GROUPS 2
-#define STREAM_THREADS (32 * STREAM_WARPS * STREAM_GROUPS)
+#define STREAM_ALL 16                       // warps of a CTA, in groups of W
+#define STREAM_THREADS (32 * STREAM_ALL)
 #define STREAM_RING(NT) ((NT) == 1 ? 4 : 3)  // chunks in a warp's ring (at 16 tokens the partial sums take the room of one)
 #define STREAM_SLOT 2176                    // 32 rows x 64 bytes, and 128 bytes of exponents
 #define STREAM_CHUNKS(NT) (32 / (NT))       // chunks of x staged at once: 64 KB
@@ -67,16 +67,16 @@ __device__ __forceinline__ uint32_t lds8(uint32_t addr) {
     return v;
 }
 
-template <int NT>
+template <int NT, int W>
 __global__ void __launch_bounds__(STREAM_THREADS, 1)
 mxfp4_stream_kernel(const MxGemm a, int units) {
     extern __shared__ __align__(16) uint8_t smem[];
     // [warp][RING] slots of weights | [group][warp][8 NT tokens][32 rows] partial sums | x: [chunk][NT][4][32 lanes] of 8 numbers
-    constexpr int RING = STREAM_RING(NT), RED = STREAM_WARPS * 8 * NT * STREAM_ROWS;
-    float *red_all = (float *)(smem + STREAM_GROUPS * STREAM_WARPS * RING * STREAM_SLOT);
-    uint4 *xs = (uint4 *)(red_all + STREAM_GROUPS * RED);
+    constexpr int GROUPS = STREAM_ALL / W, RING = STREAM_RING(NT), RED = W * 8 * NT * STREAM_ROWS;
+    float *red_all = (float *)(smem + STREAM_ALL * RING * STREAM_SLOT);
+    uint4 *xs = (uint4 *)(red_all + GROUPS * RED);
     const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = warp / STREAM_WARPS, wl = warp % STREAM_WARPS, tid = threadIdx.x & (32 * STREAM_WARPS - 1);
+    const int group = warp / W, wl = warp % W, tid = threadIdx.x & (32 * W - 1);
     float *red = red_all + group * RED;
     const uint32_t ring = smem_u32(smem) + warp * RING * STREAM_SLOT;
     const int S = gridDim.z, tiles_k = mx_tiles(a.K), blocks = a.K / MX_BLOCK;
@@ -93,8 +93,8 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
         sc += (size_t)e * mx_scale_bytes(a.N, a.K);
     } else { m_begin = blockIdx.y * 8 * NT; m_end = min(a.M, m_begin + 8 * NT); }
     const size_t pitch = a.K / 2;
-    const int first = blockIdx.x * STREAM_GROUPS + group, stride = gridDim.x * STREAM_GROUPS;
-    auto group_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * STREAM_WARPS) : "memory"); };
+    const int first = blockIdx.x * GROUPS + group, stride = gridDim.x * GROUPS;
+    auto group_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * W) : "memory"); };
 
     for (int m0 = m_begin; m0 < m_end; m0 += 8 * NT) {
         // What is copied next: chunk fc of unit fu.  Unit u is eight neighbouring rows (from 8 (u % 4)) of each quarter of a tile of 128, whose
@@ -120,14 +120,14 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
                 if (t == 0) cp_async16(ring + fs * STREAM_SLOT + 2048 + g * 16, exps + fc * MX_TILE_BYTES);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
-            fc += STREAM_WARPS;
+            fc += W;
             fs = fs + 1 == RING ? 0 : fs + 1;
         };
         for (int i = 0; i < RING - 1; i++) copy();
         int s = 0;                                                    // the slot that is used next
         bool staged = false;
-        // (both groups walk as many rounds: the barriers of the whole CTA are met by all)
-        for (int u0 = blockIdx.x * STREAM_GROUPS; u0 < units; u0 += stride) {
+        // (all groups walk as many rounds: the barriers of the whole CTA are met by all)
+        for (int u0 = blockIdx.x * GROUPS; u0 < units; u0 += stride) {
             const int u = u0 + group;
             const bool live = u < units;
             float sum[2][NT][4];
@@ -160,7 +160,7 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
                     staged = true;
                 }
                 if (!live) continue;
-                for (int c = s0 + wl; c < s1; c += STREAM_WARPS) {
+                for (int c = s0 + wl; c < s1; c += W) {
                     asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
                     __syncwarp();                                     // the exponents were copied by other lanes
                     const uint32_t slot = ring + s * STREAM_SLOT;
@@ -206,7 +206,7 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
                     s = s + 1 == RING ? 0 : s + 1;
                 }
             }
-            // ---- sums of the eight warps, then of the cluster's CTAs
+            // ---- sums of the group's warps, then of the cluster's CTAs
             const int total = live ? min(8 * NT, m_end - m0) * STREAM_ROWS : 0;
             auto store = [&](int q, float v) {
                 const int rl = q % STREAM_ROWS, n = (u >> 2) * 128 + (rl >> 3) * 32 + (u & 3) * 8 + (rl & 7);
@@ -221,10 +221,10 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
                         for (int j = 0; j < 4; j++)
                             red[(wl * 8 * NT + n * 8 + 2 * t + (j & 1)) * STREAM_ROWS + (2 * i + (j >> 1)) * 8 + g] = sum[i][n][j];
                 group_sync();
-                for (int q = tid; q < total; q += 32 * STREAM_WARPS) {
+                for (int q = tid; q < total; q += 32 * W) {
                     float v = red[q];
 #pragma unroll
-                    for (int z = 1; z < STREAM_WARPS; z++) v += red[z * 8 * NT * STREAM_ROWS + q];
+                    for (int z = 1; z < W; z++) v += red[z * 8 * NT * STREAM_ROWS + q];
                     if (S == 1) store(q, v); else red[q] = v;
                 }
                 group_sync();                                         // before the next unit's sums
@@ -232,7 +232,7 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
             if (S > 1) {
                 cluster_sync_all();
                 const uint32_t red0 = smem_u32(red);
-                for (int q = blockIdx.z * 32 * STREAM_WARPS + tid; q < total; q += 32 * STREAM_WARPS * S) {
+                for (int q = blockIdx.z * 32 * W + tid; q < total; q += 32 * W * S) {
                     float part[8];
 #pragma unroll
                     for (int z = 0; z < 8; z++) part[z] = z < S ? ld_dsmem_f32(red0 + q * 4, z) : 0.f;
@@ -249,26 +249,51 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
     }
 }
 
-template <int NT>
-static int launch_stream(MxGemm a, int y, int busy /* of the y, that have rows */, cudaStream_t stream) {
-    constexpr int fixed = STREAM_GROUPS * STREAM_WARPS * (STREAM_RING(NT) * STREAM_SLOT + 8 * NT * STREAM_ROWS * 4);
-    static FgPerDevice configured;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(mxfp4_stream_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + 65536);
-        if (e != cudaSuccess) return (int)e;
+template <int NT, int W>
+struct MxStreamForm {
+    static constexpr int groups = STREAM_ALL / W, fixed = STREAM_ALL * (STREAM_RING(NT) * STREAM_SLOT + 8 * NT * STREAM_ROWS * 4), room_bytes = fixed + 65536;
+    static int setup() {
+        static FgPerDevice configured;
+        return fg_needs_setup(configured) ? (int)cudaFuncSetAttribute(mxfp4_stream_kernel<NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, room_bytes) : 0;
     }
-    static MxClusters known;
-    auto room = [&](int S) { return mx_clusters(known, mxfp4_stream_kernel<NT>, STREAM_THREADS, fixed + 65536, S); };
-    const int tiles_k = mx_tiles(a.K), units = 4 * mx_tiles(a.N);
-    // K over a cluster: until x fits at once, and while there are too few units for the SMs and each warp keeps a chunk
-    int S = 1;
-    while (S < 8 && (tiles_k > S * STREAM_CHUNKS(NT) || ((long long)units * busy <= room(2 * S) * STREAM_GROUPS && tiles_k > S * STREAM_WARPS))) S *= 2;
-    a.chunks_per_split = (tiles_k + S - 1) / S;
-    const int staged = a.chunks_per_split < STREAM_CHUNKS(NT) ? a.chunks_per_split : STREAM_CHUNKS(NT);
-    const int pairs = (units + STREAM_GROUPS - 1) / STREAM_GROUPS;
-    int gx = room(S) / busy;                                         // as many CTAs as fit at once
-    gx = gx < 1 ? 1 : gx > pairs ? pairs : gx;
-    return mx_launch(mxfp4_stream_kernel<NT>, dim3(gx, y, S), STREAM_THREADS, fixed + staged * NT * 2048, dim3(1, 1, S), stream, a, units);
+    static int room(int S) {                                         // CTAs (a cluster of S each) that fit at once
+        static MxClusters known;
+        return mx_clusters(known, mxfp4_stream_kernel<NT, W>, STREAM_THREADS, room_bytes, S);
+    }
+    static int width(int S, int busy, int units) {                   // CTAs along the units
+        const int most = (units + groups - 1) / groups, gx = room(S) / busy;
+        return gx < 1 ? 1 : gx > most ? most : gx;
+    }
+    // The split of K that finishes first, in us: rounds of units times a warp's chunks and the sums behind them.  Fitted to us | us with groups of eight | four
+    // warps, eight rows: 28,672 x 4,096: 23.5 | 22.6; 16,384 x 2,048: 9.6 | 8.9; 4,096 x 14,336: 16.6 | 13.9; 8,192 x 2,048: 6.0 | 6.6 (it splits K);
+    // 2,048 x 8,192: 7.4 | 9.3; one row of 128,256 x 2,048: 42.5 | 35.1 (sums of half as many warps, half as often).
+    static double plan(int units, int tiles_k, int busy, int &S) {
+        double best = 1e30;
+        if (setup()) cudaGetLastError();                             // (its launch reports it)
+        for (int s = 1; s <= 8; s *= 2) {
+            if (s < 8 && tiles_k > s * STREAM_CHUNKS(NT)) continue;  // until x fits at once
+            if (best < 1e30 && tiles_k <= s / 2 * W) break;          // each warp keeps a chunk
+            const int chunks = ((tiles_k + s - 1) / s + W - 1) / W;
+            const long long lanes = (long long)width(s, busy, units) * groups, rounds = (units + lanes - 1) / lanes;
+            const double cost = rounds * (1.1 * chunks + (W == 8 ? 0.55 : 0.2) + (s > 1 ? (W == 8 ? 0.35 : 0.45) * s : 0.0));
+            if (cost < best) { best = cost; S = s; }
+        }
+        return best;
+    }
+    static int launch(MxGemm a, int y, int busy, int units, int S, cudaStream_t stream) {
+        const int rc = setup(), tiles_k = mx_tiles(a.K);
+        if (rc) return rc;
+        a.chunks_per_split = (tiles_k + S - 1) / S;
+        const int staged = a.chunks_per_split < STREAM_CHUNKS(NT) ? a.chunks_per_split : STREAM_CHUNKS(NT);
+        return mx_launch(mxfp4_stream_kernel<NT, W>, dim3(width(S, busy, units), y, S), STREAM_THREADS, fixed + staged * NT * 2048, dim3(1, 1, S), stream, a, units);
+    }
+};
+template <int NT>
+static int launch_stream(const MxGemm &a, int y, int busy /* of the y, that have rows */, cudaStream_t stream) {
+    const int units = 4 * mx_tiles(a.N), tiles_k = mx_tiles(a.K);
+    int s8 = 1, s4 = 1;
+    const double eight = MxStreamForm<NT, 8>::plan(units, tiles_k, busy, s8), four = MxStreamForm<NT, 4>::plan(units, tiles_k, busy, s4);
+    return four < eight ? MxStreamForm<NT, 4>::launch(a, y, busy, units, s4, stream) : MxStreamForm<NT, 8>::launch(a, y, busy, units, s8, stream);
 }
 
 // ---------------------------------------------------------------------------- more rows: weights through tensor memory

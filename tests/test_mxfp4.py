@@ -308,6 +308,24 @@ def test_many_tiles_a_processor(form, bn):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 40001, 96), (8, 19999, 544), (3, 40000, 2048), (5, 4099, 14336), (2, 700, 40000), (20, 9001, 1056)])
+def test_few_rows_over_many_units_and_long_rows(m, n, k):
+    """Sizes for which the kernel for few rows takes units with fewer warps, and splits long rows over a cluster; the same call gives the same bits."""
+    w, numbers = _matrix(n, k, 61)
+    x = _rows(m, k, 62)
+    odd = torch.zeros(m, k + 1, dtype=torch.bfloat16, device="cuda")                       # (rows that TMA cannot address, for more than eight)
+    odd[:, :k] = x.cuda()
+    want, slack = plain.product(x, numbers)
+    for rows in (x.cuda(), odd[:, :k]):
+        out = ops.gemm_mxfp4(rows, w, out_dtype=torch.float32)
+        plain.check(out, want, slack)
+        assert torch.equal(out, ops.gemm_mxfp4(rows, w, out_dtype=torch.float32))
+        both = torch.full((m, n), 1.5, device="cuda")
+        ops.gemm_mxfp4(rows, w, out=both, accumulate=True)
+        assert torch.equal(both, out + 1.5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 5, 16, 40, 130, 300])
 def test_contraction_on_strided_rows(m):
     n, k = 333, 544
