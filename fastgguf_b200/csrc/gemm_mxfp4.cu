@@ -435,6 +435,9 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     if (threadIdx.x == 64) { tma_prefetch_map(&tmX); tma_prefetch_map(&tmW); }
     pdl_wait();                                     // (before tensor memory is allocated: no kernel in front holds any then)
     pdl_launch_dependents();
+    // the partner runs, and its barriers exist, before a pair allocates tensor memory together or anything arrives on them; its own tensor memory is
+    // there when its first arrival on full says so
+    if (PAIR) { __syncthreads(); cluster_sync_all(); }
     if (warp == 1) { if (PAIR) tc_alloc_pair(smem_u32(&tmem_base_s), 512); else tc_alloc(smem_u32(&tmem_base_s), 512); }
     if (a.g.offsets && warp == 0) {                 // tiles of x in front of each expert's run
         int sum = 0;
@@ -452,7 +455,6 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
-    if (PAIR) cluster_sync_all();                   // the partner's barriers exist before anything arrives on them
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;
     const int n_tiles = a.g.offsets ? cum[a.g.experts] * a.tiles_n : a.n_tiles;
@@ -482,6 +484,9 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         }
         if (rank == 0)                              // copies in flight land before the CTA exits
             for (int j = max(0, g - xs); j < g; j++) mbar_wait(full0 + 8 * (j % TILE_SLOTS), (j / TILE_SLOTS) & 1);
+        // so do the last commits' arrivals, which come from the tensor core, a pair's from the leader's SM
+        for (int j = max(0, g - TILE_SLOTS); j < g; j++) mbar_wait(done0 + 8 * (j % TILE_SLOTS), (j / TILE_SLOTS) & 1);
+        __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (a pair's leader alone)
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)((PAIR ? 2 : 1) * TILE_ROWS >> 4) << 24);
@@ -512,6 +517,7 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
             if (elect_one()) { if (PAIR) tc_commit_pair(tfull); else tc_commit(tfull); }      // also after an error: the epilogue is not left waiting
             __syncwarp();
         }
+        if (rank == 0 && i > 0) mbar_wait_warp(tempty, (i - 1) & 1);                         // the last tile's arrivals, the partner's among them
     } else if (warp == 2) {
         // ------------------------------------------------------------ weights and exponents
         int s = 0, ph = 0, issued = 0;

@@ -87,6 +87,9 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
         }
         for (int j = max(0, issued - stages); j < issued; j++)      // copies in flight land before the CTA exits
             mbar_wait(full0 + 8 * (j % stages), (j / stages) & 1);
+        for (int j = max(0, issued - stages); j < issued; j++)      // so do the last commits' arrivals
+            mbar_wait(empty0 + 8 * (j % stages), (j / stages) & 1);
+        __syncwarp();
     } else if (warp == 1) {
         // instruction descriptor: both operands e2m1, exponents as bytes; bits 4 and 29 name the half word of exponents a step reads
         const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(bn >> 3) << 17) | (1u << 23) | ((uint32_t)(BOTH_ROWS >> 4) << 24);
