@@ -684,8 +684,9 @@ static void tile_plan(int M, int N, int K, bool &pair, int &bn, int &S) {
     double best = 1e30;
     for (int p = 0; p < 2; p++) {
         const int rows = p ? 2 * TILE_ROWS : TILE_ROWS, tiles_n = (N + rows - 1) / rows, units = p ? n_sm / 2 : n_sm;
-        for (int b = 16; b <= 256; b += 16) {
-            if (b > 16 && b - 16 >= M) break;                        // wider than the rows there are
+        const int step = p ? 32 : 16;                                // (a CTA of a pair brings whole groups of 16 tokens)
+        for (int b = step; b <= 256; b += step) {
+            if (b > step && b - step >= M) break;                    // wider than the rows there are
             const long long tiles = (long long)((M + b - 1) / b) * tiles_n;
             for (int s = 1; s <= (p ? 1 : 8); s++) {
                 if (s > 1 && tiles > mx_clusters(known, mxfp4_tile_kernel<false>, TILE_THREADS, TILE_SMEM, s)) continue;
@@ -711,7 +712,7 @@ static int mx_check(const MxGemm &a) {
     return 0;
 }
 
-// form: 0 by the rule; 1 the kernel for few rows, 2 tiles, 3 tiles of pairs of CTAs, with `bn` tokens a tile (a multiple of 16) and K split
+// form: 0 by the rule; 1 the kernel for few rows, 2 tiles, 3 tiles of pairs of CTAs, with `bn` tokens a tile (a multiple of 16, of pairs 32) and K split
 // over `splits` CTAs (form 2): for tests and measurements
 extern "C" int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
                                  int M, int N, int K, int form, int bn, int splits, cudaStream_t stream) {
@@ -725,7 +726,7 @@ extern "C" int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, co
         form = M > 8 && tile_ok(a) ? 2 : 1;
         if (form == 2) tile_plan(M, N, K, pair, bn, splits);
         if (pair) form = 3;
-    } else if (form < 1 || form > 3 || (form > 1 && (!tile_ok(a) || bn < 16 || bn > 256 || bn % 16 || splits < 1 || splits > 8 || (form == 3 && splits > 1))))
+    } else if (form < 1 || form > 3 || (form > 1 && (!tile_ok(a) || bn < 16 || bn > 256 || bn % 16 || splits < 1 || splits > 8 || (form == 3 && (splits > 1 || bn % 32)))))
         return FG_ERR_BAD_SIZE;
     if (form == 2) return launch_tiles<false>(a, bn, splits, stream);
     if (form == 3) return launch_tiles<true>(a, bn, 1, stream);

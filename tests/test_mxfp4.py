@@ -127,7 +127,7 @@ def test_calls_that_do_not_fit_are_refused_before_a_launch(no_device_check):
             call()
 
 
-def test_launchers_refuse_rows_beyond_31_bits(no_device_check):
+def test_launchers_refuse_rows_beyond_31_bits_and_other_widths(no_device_check):
     """Before they touch the device or the memory (the addresses here are none)."""
     from ctypes import c_void_p
     L, refused, most, at = ops.lib("mx"), 10002, 2 ** 31 - 1, c_void_p(1 << 20)          # (FG_ERR_BAD_SIZE)
@@ -136,8 +136,11 @@ def test_launchers_refuse_rows_beyond_31_bits(no_device_check):
         assert L.fg_gemm_mxfp4(at, 32, at, at, at, 1, N, 0, M, N, 32, None) == refused
         for form in (1, 2, 3):
             assert L.fg_gemm_mxfp4_ext(at, 32, at, at, at, 1, N, 0, M, N, 32, form, 16, 1, None) == refused
+            assert L.fg_gemm_mxfp4_ext(at, 32, at, at, at, 1, N, 0, M, N, 32, form, 32, 1, None) == refused
         assert L.fg_gemm_mxfp4_both(at, at, at, at, at, 1, N, 0, M, N, 32, None) == refused
         assert L.fg_gemm_mxfp4_grouped(at, 32, at, at, at, 2, at, 1, N, 0, M, N, 32, None) == refused
+    for bn in (0, 8, 16, 48, 240, 272):                                                       # a pair's tiles are multiples of 32 tokens
+        assert L.fg_gemm_mxfp4_ext(at, 32, at, at, at, 1, 64, 0, 64, 64, 32, 3, bn, 1, None) == refused
     assert L.fg_gemm_mxfp4_grouped(at, 32, at, at, at, 1000, at, 1, 3000000, 0, 4, 3000000, 32, None) == refused       # 3 10^9 rows of all experts
 
 
@@ -287,7 +290,7 @@ def _named(x, w, form, bn=16, splits=1, dtype=torch.float32):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("form,bn,splits", [(1, 16, 1), (2, 16, 1), (2, 48, 3), (2, 112, 8), (2, 256, 1), (2, 256, 2), (3, 16, 1), (3, 80, 1), (3, 240, 1), (3, 256, 1)])
+@pytest.mark.parametrize("form,bn,splits", [(1, 16, 1), (2, 16, 1), (2, 48, 3), (2, 112, 8), (2, 256, 1), (2, 256, 2), (3, 32, 1), (3, 96, 1), (3, 224, 1), (3, 256, 1)])
 @pytest.mark.parametrize("m,n,k", [(1, 100, 32), (70, 129, 96), (40, 513, 1056), (300, 384, 2080), (777, 1000, 160)])
 def test_every_kernel_at_every_width(form, bn, splits, m, n, k):
     x, (w, numbers) = _rows(m, k, m + n).cuda(), _matrix(n, k, n + k)
