@@ -39,7 +39,7 @@ __device__ __forceinline__ uint32_t to_e2m1x2(float lo, float hi) {
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-mxfp4_quantize_kernel(const T *__restrict__ x, long long ldx, long long x_stride, uint8_t *__restrict__ data, uint8_t *__restrict__ scales, int R,
+mxfp4_quantize_kernel(const T *x, long long ldx, long long x_stride, uint8_t *__restrict__ data, uint8_t *__restrict__ scales, int R,
                       int K, int tiles_r, int vec) {
     constexpr int V = 32 / sizeof(T), THREADS = 128 / V, ROWS = 256 / THREADS;      // numbers a piece, threads a row, rows a pass of the CTA
     __shared__ __align__(16) uint8_t tile[MX_TILE_BYTES];
@@ -49,6 +49,8 @@ mxfp4_quantize_kernel(const T *__restrict__ x, long long ldx, long long x_stride
     pdl_wait();
     pdl_launch_dependents();
     __syncthreads();
+    // (the loads are plain asm, so that passes overlap: an address that is known only here keeps them behind the wait)
+    asm volatile("" : "+l"(x) : : "memory");
     const T *src = x + (size_t)mat * x_stride + k;
     uint8_t *dst = data + (size_t)mat * R * (K / 2) + k / 2;
     // (every thread walks all passes: the shuffles name all lanes)
@@ -135,13 +137,14 @@ __device__ __forceinline__ void store8(bf16 *p, bool vec, const float (&v)[8]) {
 // pieces 0 .. total - 1 of the rows from r0 on; `over` is 2^64 / (pieces a row) rounded up, by which a piece's row is one multiplication
 template <typename T>
 __global__ void __launch_bounds__(256)
-mxfp4_rows_kernel(const uint8_t *__restrict__ data, const uint8_t *__restrict__ scales, const int *__restrict__ rows, T *__restrict__ out,
+mxfp4_rows_kernel(const uint8_t *data, const uint8_t *scales, const int *rows, T *__restrict__ out,
                   long long ldo, int r0, unsigned total, unsigned long long over, int R, int K, float scale, int vec) {
     const int tiles_k = mx_tiles(K);
     const unsigned at0 = blockIdx.x * (256 * ROWS_PIECES) + threadIdx.x, per_row = K / 8;
     uint32_t w[ROWS_PIECES], e[ROWS_PIECES];
     long long to[ROWS_PIECES];
     pdl_wait();
+    asm volatile("" : "+l"(data), "+l"(scales), "+l"(rows) : : "memory");       // (addresses known only here keep the loads behind the wait)
 #pragma unroll
     for (int p = 0; p < ROWS_PIECES; p++) {
         const unsigned at = at0 + p * 256;
