@@ -304,7 +304,7 @@ static int launch_stream(const MxGemm &a, int y, int busy /* of the y, that have
 //
 //   warp 0      tokens: two boxes of 64 numbers a stage, a ring of up to four
 //   warp 1      MMA issuer: eight 128 x BN x 16 a stage; its commit frees the stage's tokens and its slot of tensor memory (four of 64 columns)
-//   warp 2      weights: 64 bytes a row and 512 bytes of exponents a stage, a ring of six
+//   warp 2      weights: 64 bytes a row and 512 bytes of exponents a stage, a ring of eight
 //   warps 3-18  four sets of four, a set to a slot: unpack every fourth stage, and at a tile's end a quarter of its epilogue.  The first
 //               stages of the next tile are unpacked BEFORE a tile's epilogue: the tensor core goes on meanwhile.
 // Unpacking is bound by the integer pipe when enough warps hide the waits around it: with two warps a scheduler, half a stage each, a
@@ -321,13 +321,16 @@ static int launch_stream(const MxGemm &a, int y, int busy /* of the y, that have
 #define TILE_THREADS 608
 #define TILE_W_BYTES (TILE_ROWS * TILE_K / 2)
 #define TILE_W_STAGE (TILE_W_BYTES + 1024)
-#define TILE_W_STAGES 6
+// A set waits on a place of this ring by parity, and knows only of its own stages that they have come: a place has to be one set's, or a copy that
+// is overtaken by a later one leaves the place a phase behind and the wait passes early.
+#define TILE_W_STAGES 8
 #define TILE_SLOTS 4            // stages in tensor memory, 64 columns each, behind the accumulator's 256
 #define TILE_AHEAD 3            // stages of the next tile that are unpacked before a tile's epilogue
 #define TILE_MAX_EXPERTS 1024
 #define TILE_SMEM (221 * 1024)
 #define TILE_UNPACK 650         // SM cycles a stage takes at few tokens: its unpacking
 
+static_assert(TILE_W_STAGES % TILE_SLOTS == 0, "a place of the weights' ring belongs to one set of unpacking warps");
 struct MxTiles {
     MxGemm g;
     int bn, xs, tiles_m, tiles_n, n_tiles;          // tokens a tile, depth of their ring (grouped: tiles_m and n_tiles follow from the offsets)

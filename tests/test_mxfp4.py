@@ -639,6 +639,31 @@ def test_two_calls_at_once():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 2048), (12, 28672, 4096), (40, 2048, 4096), (200, 8192, 2048)])
+def test_beside_a_stream_that_keeps_memory_busy(m, n, k):
+    """Every form starts and ends many times while another stream quantises and reads large matrices: the same bits as alone."""
+    w, _ = _matrix(n, k, 71)
+    stack = Mxfp4(w.data.view(4, n // 4, k // 2), w.scales.view(4, n // 512, -1, 32, 4, 4))
+    x, other = _rows(m, k, 72).cuda(), torch.randn(8192, 4096, device="cuda")
+    q, offsets = ops.mxfp4_quantize(x), torch.tensor([0, m // 3, m // 3, m, m], dtype=torch.int32, device="cuda")
+    calls = [lambda: ops.gemm_mxfp4(x, w), lambda: ops.gemm_mxfp4_both(q, w), lambda: ops.gemm_mxfp4_grouped(x, stack, offsets)]
+    calls += [lambda f=f, b=b, z=z: _named(x, w, f, b, z) for f, b, z in [(2, 16, 1), (2, 48, 2), (2, 256, 1), (3, 32, 1), (3, 256, 1)] if z == 1 or n <= 2048]
+    alone = [c().clone() for c in calls]
+    beside, mine = torch.cuda.Stream(), torch.cuda.Stream()
+    beside.wait_stream(torch.cuda.current_stream())
+    mine.wait_stream(torch.cuda.current_stream())
+    for _ in range(15):
+        with torch.cuda.stream(beside):
+            for _ in range(4):
+                ops.mxfp4_rows(ops.mxfp4_quantize(other))
+        with torch.cuda.stream(mine):
+            for c, want in zip(calls, alone):
+                assert torch.equal(c(), want)
+    torch.cuda.synchronize()
+    ops.raise_on_device_error("beside another stream")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("which", ["tiles", "tiles split", "pairs", "both"])
 def test_a_wait_that_runs_out_ends_the_kernel_and_the_next_is_correct(which):
     """The first copy of tokens is left out and waits are shortened to about a millisecond: the kernel gives up, raises its error flag, frees its tensor
@@ -646,6 +671,7 @@ def test_a_wait_that_runs_out_ends_the_kernel_and_the_next_is_correct(which):
     import time
     from ctypes import c_int, c_longlong
     m, n, k = 100, 300, 2048
+    bn = 96 if which == "pairs" else 112
     w, numbers = _matrix(n, k, 8)
     x = _rows(m, k, 9)
     q, xd = ops.mxfp4_quantize(x.cuda()), x.cuda()
@@ -653,7 +679,7 @@ def test_a_wait_that_runs_out_ends_the_kernel_and_the_next_is_correct(which):
     def call():
         if which == "both":
             return ops.gemm_mxfp4_both(q, w, out_dtype=torch.float32)
-        return _named(xd, w, 3 if which == "pairs" else 2, 112, 4 if which == "tiles split" else 1).clone()
+        return _named(xd, w, 3 if which == "pairs" else 2, bn, 4 if which == "tiles split" else 1).clone()
 
     error, hook = ops.lib("mx").fg_gemm_mxfp4_error, ops.lib("mx").fg_gemm_mxfp4_test_hook
     hook.argtypes, hook.restype = [c_longlong, c_int], c_int
@@ -669,7 +695,7 @@ def test_a_wait_that_runs_out_ends_the_kernel_and_the_next_is_correct(which):
         else:
             out = torch.empty(m, n, device="cuda")
             ops.lib("mx").fg_gemm_mxfp4_ext(xd.data_ptr(), k, w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), 0, n, 0, m, n, k, 3 if which == "pairs" else 2,
-                                            112, 4 if which == "tiles split" else 1, torch.cuda.current_stream().cuda_stream)
+                                            bn, 4 if which == "tiles split" else 1, torch.cuda.current_stream().cuda_stream)
         torch.cuda.synchronize()
         assert time.time() - t0 < 2.0
         with pytest.raises(KernelError, match="wait ran out"):
