@@ -40,7 +40,7 @@ __device__ __forceinline__ void mx_store(const MxGemm &a, int m, int n, float v)
 // on an SM, with no registers held for them), so the ring needs no barrier.
 //
 // What bounds it: instructions.  At the memory's rate an SM gets a chunk's 2,176 bytes of 32 rows every 92 cycles, in which its four
-// schedulers issue 368; unpacking them takes 192, the MMAs, loads and addresses some 70.  Measured: 8 x 28,672 x 4,096 22.6 us (2.8 TB/s), one row of
+// schedulers issue 368; unpacking them takes 192, the MMAs, loads and addresses some 70.  Measured: 8 x 28,672 x 4,096 22.5 us (2.8 TB/s), one row of
 // 128,256 x 2,048 35.1 (4.0).  Sixteen warps do not hide all of their waits: with two groups of eight (23.5 us) the schedulers issued in 54 % of active
 // cycles, DRAM was at 29 %.
 //
@@ -310,7 +310,7 @@ static int launch_stream(const MxGemm &a, int y, int busy /* of the y, that have
 // Unpacking is bound by the integer pipe when enough warps hide the waits around it: with two warps a scheduler, half a stage each, a
 // stage's took 1,500 cycles beside the 1,024 of its MMAs at 256 tokens (2,048 x 8,192 x 4,096: 133 us; with four: 94).  At few tokens a stage
 // takes some 650 cycles: unpacking and the chain from a free slot to the next full one, beside MMAs of 46 cycles each.
-// Measured: 77 x 8,191 x 2,080 9.5 us; 256 x 8,192 x 4,096 17.4 us (988 TFLOP/s); 2,048 x 14,336 x 4,096 158 us (1,519 TFLOP/s) in a short run, 181 at the
+// Measured: 77 x 8,191 x 2,080 9.5 us; 256 x 8,192 x 4,096 17.3 us (995 TFLOP/s); 2,048 x 14,336 x 4,096 162 us (1,482 TFLOP/s) in a short run, 181 at the
 // power limit; at 2,048 x 28,672 x 4,096 the tensor pipe is busy in 86 % of active cycles.
 //
 // One CTA an SM walks the tiles.  PAIR: two CTAs of a cluster take 256 weight rows x BN tokens (tcgen05.mma.cta_group::2); each unpacks its

@@ -111,8 +111,8 @@ extern "C" int fg_mxfp4_quantize(const void *x, int dtype, long long ldx, long l
 // ---------------------------------------------------------------------------- rows
 // out[i] = scale * row rows[i] (null: row i).  A piece is eight numbers, which lie in one block: four bytes in, 16 or 32 out.  A thread takes four
 // pieces, 256 apart, and asks for all of them before it converts the first.  The number itself is exact in either type; a scale other than 1 rounds
-// once.  A row index outside the matrix gives a row of NaN.  14,336 x 4,096: 42.8 us to float32 (6.2 TB/s), 35.2 to bfloat16 (4.2); 4,001 picked rows
-// of 2,048 6.8 us (5.5).
+// once.  A row index outside the matrix gives a row of NaN.  14,336 x 4,096: 42.9 us to float32 (6.2 TB/s), 37.7 to bfloat16 (3.9); 4,001 picked rows
+// of 2,048 6.9 us (5.4).
 #define ROWS_PIECES 4
 __device__ __forceinline__ void store8(float *p, bool vec, const float (&v)[8]) {
     if (vec)
