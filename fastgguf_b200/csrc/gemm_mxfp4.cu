@@ -54,7 +54,10 @@ __device__ __forceinline__ void mx_store(const MxGemm &a, int m, int n, float v)
 #define STREAM_SLOT 2176                    // 32 rows x 64 bytes, and 128 bytes of exponents
 #define STREAM_CHUNKS(NT) (32 / (NT))       // chunks of x staged at once: 64 KB
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+// sixteen bytes, of which the first `have` are read, the others zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t have = 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
+}
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -98,8 +101,8 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
 
     for (int m0 = m_begin; m0 < m_end; m0 += 8 * NT) {
         // What is copied next: chunk fc of unit fu.  Unit u is eight neighbouring rows (from 8 (u % 4)) of each quarter of a tile of 128, whose
-        // exponents are 128 neighbouring bytes.  Rows past the last read that one (their sums are not stored), blocks past the end of K the row's
-        // first (x is zero there).
+        // exponents are 128 neighbouring bytes.  Rows past the last read that one (their sums are not stored).  Blocks past the end of K get codes of zero:
+        // their exponents are padding, any byte but 255, and a number under 253 or 254 may be infinite, which the zeros of x do not cancel.
         int fu = first - stride, fc = c_end, fs = 0;
         const uint8_t *row[4], *exps = nullptr;
         auto copy = [&] {
@@ -113,10 +116,11 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
                 }
             }
             if (fu < units && fc < c_end) {
-                const int at = fc * 4 + t < blocks ? fc * 64 : -t * 16;
+                const bool there = fc * 4 + t < blocks;
+                const int at = there ? fc * 64 : -t * 16;
                 const uint32_t dst = ring + fs * STREAM_SLOT + lane * 16;
 #pragma unroll
-                for (int j = 0; j < 4; j++) cp_async16(dst + j * 512, row[j] + at);
+                for (int j = 0; j < 4; j++) cp_async16(dst + j * 512, row[j] + at, there ? 16 : 0);
                 if (t == 0) cp_async16(ring + fs * STREAM_SLOT + 2048 + g * 16, exps + fc * MX_TILE_BYTES);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
