@@ -87,7 +87,6 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
     const bool in_parts = c_end - c_begin > STREAM_CHUNKS(NT);
     const uint8_t *w = a.w, *sc = a.sc;
     pdl_wait();
-    pdl_launch_dependents();
     int m_begin, m_end;
     if (a.offsets) {
         const int e = blockIdx.y;
@@ -441,7 +440,6 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     }
     if (threadIdx.x == 64) { tma_prefetch_map(&tmX); tma_prefetch_map(&tmW); }
     pdl_wait();                                     // (before tensor memory is allocated: no kernel in front holds any then)
-    pdl_launch_dependents();
     // the partner runs, and its barriers exist, before a pair allocates tensor memory together or anything arrives on them; its own tensor memory is
     // there when its first arrival on full says so
     if (PAIR) { __syncthreads(); cluster_sync_all(); }

@@ -53,7 +53,6 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
     }
     if (threadIdx.x == 64) { tma_prefetch_map(&tmX); tma_prefetch_map(&tmW); }
     pdl_wait();                                     // (before tensor memory is allocated: no kernel in front holds any then)
-    pdl_launch_dependents();
     if (warp == 1) tc_alloc(smem_u32(&tmem_base_s), 512);
     tc_fence_before();
     __syncthreads();

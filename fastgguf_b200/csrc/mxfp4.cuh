@@ -66,9 +66,9 @@ __device__ __forceinline__ void mx_unpack32(const uint4 &d, uint32_t e, uint32_t
 
 // ---------------------------------------------------------------------------- launches
 // Dependent launches: a kernel of this library waits for its predecessor before it touches any memory (weights too: the quantiser may just have
-// written them) and only then releases its successor, so that one never runs beside the kernel before its predecessor.  The release
-// saves the drain and the launch between two small kernels.  mxfp4_rows, whose output may be weights that a contraction reads before its wait, does not
-// release early.
+// written them).  Only the quantiser releases its successor before it ends, behind that wait, so that one never runs beside the kernel before its
+// predecessor.  Readers and contractions do not: what they write may be the weights of a bfloat16 or float32 contraction (the keys of scores, a product of
+// factors), which the next kernel of the stream, or the one behind that, fetches before its own wait.  Codes and exponents are read by this library alone.
 template <typename... KArgs, typename... Args>
 static inline int mx_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, dim3 cluster, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};

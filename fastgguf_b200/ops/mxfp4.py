@@ -9,6 +9,8 @@ A number is a sign, two exponent bits and one mantissa bit (0, 0.5, 1, 1.5, 2, 3
   [r // 128, b // 4, r % 32, r // 32 % 4, b % 4].  Exponents of rows and blocks past the matrix are padding, any byte but 255.
 
 ``Mxfp4.from_exponents`` takes exponents row by row, ``exponents`` gives them so.
+
+What a call writes may be any input of the next call on the stream, the weights of another operator included.
 """
 from __future__ import annotations
 

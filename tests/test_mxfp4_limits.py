@@ -54,3 +54,78 @@ def test_padding_exponents_change_no_bit(m, k):
     for byte in (126, 252, 253, 254):
         for i, (got, zero) in enumerate(zip(results(byte), want)):
             assert torch.equal(got, zero), (byte, i)
+
+
+# ------------------------------------------------------------------------------ outputs as the weights of the next kernel
+def test_only_the_quantiser_releases_its_successor_early():
+    """What the other kernels write may be weights, which a bfloat16 or float32 contraction fetches before it waits for the kernels in front of it."""
+    import os
+    import re
+    from fastgguf_b200.csrc import build
+    releasing = set()
+    for name in ("mxfp4.cu", "mxfp4.cuh", "mxfp4_tc.cuh", "gemm_mxfp4.cu", "gemm_mxfp4_both.cuh"):
+        with open(os.path.join(build.CSRC_DIR, name)) as f:
+            code = re.sub(r"//[^\n]*", "", f.read())
+        for part in code.split("__global__")[1:]:
+            if "pdl_launch_dependents" in part or "griddepcontrol.launch_dependents" in part:
+                releasing.add(re.search(r"(\w+_kernel)\(", part).group(1))
+    assert releasing == {"mxfp4_quantize_kernel"}
+
+
+def _random(n, k, seed, lead=()):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*lead, n, k, generator=g, device="cuda") * k ** -0.5).bfloat16()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("n", [8, 48, 640, 2048])
+def test_an_output_is_the_weight_of_the_next_contraction(n, rows):
+    """The contractions write W, the next kernel of the stream (or the one behind that) reads it as its weights: as if the device were waited for in between."""
+    from fastgguf_b200.ops import fast_gemm
+    k, mid = 1024, 512
+    w = ops.mxfp4_quantize(_random(mid, k, 1))
+    stack = ops.mxfp4_quantize(_random(mid, k, 2, (2,)))
+    cut = torch.tensor([0, n // 3, n], dtype=torch.int32, device="cuda")
+    inputs = [_random(n, k, 10 + i) for i in range(6)]
+    packed = [ops.mxfp4_quantize(t) for t in inputs]
+    a, a32 = _random(rows, mid, 3), _random(rows, mid, 4).float()
+    other = _random(256, mid, 5)
+    made, made32 = torch.zeros(n, mid, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, mid, device="cuda")
+    writers = [lambda i, out: ops.gemm_mxfp4(inputs[i], w, out=out), lambda i, out: ops.gemm_mxfp4_both(packed[i], w, out=out),
+               lambda i, out: ops.gemm_mxfp4_grouped(inputs[i], stack, cut, out=out)]
+    f32 = fast_gemm.gemm_f32_stream if rows <= 16 else fast_gemm.gemm_f32
+
+    def chain(write, i, wait):
+        write(i, made)
+        if wait:
+            torch.cuda.synchronize()
+        got = [fast_gemm.gemm_tc(a, made)]
+        write((i + 1) % len(inputs), made)
+        if wait:
+            torch.cuda.synchronize()
+        fast_gemm.gemm_tc(a, other)                          # (a kernel between that releases its successor before it waits)
+        got.append(fast_gemm.gemm_tc(a, made))
+        write(i, made32)
+        if wait:
+            torch.cuda.synchronize()
+        got.append(f32(a32, made32))
+        return got
+
+    for write in writers:
+        want = [[t.clone() if t is not None else None for t in chain(write, i, True)] for i in range(len(inputs))]
+        assert want[0][0] is not None and not torch.equal(want[0][0], want[1][0])
+        got = [chain(write, i, False) for _ in range(10) for i in range(len(inputs))]
+        torch.cuda.synchronize()
+        for j, g in enumerate(got):
+            for x, y in zip(g, want[j % len(inputs)]):
+                assert (x is None and y is None) or torch.equal(x, y)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            recorded = [chain(write, i, False) for i in range(len(inputs))]
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        for g, y in zip(recorded, want):
+            assert all((p is None and q is None) or torch.equal(p, q) for p, q in zip(g, y))
+    ops.raise_on_device_error("chains")
