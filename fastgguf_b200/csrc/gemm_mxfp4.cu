@@ -120,7 +120,7 @@ mxfp4_stream_kernel(const MxGemm a, int units) {
                 const uint32_t dst = ring + fs * STREAM_SLOT + lane * 16;
 #pragma unroll
                 for (int j = 0; j < 4; j++) cp_async16(dst + j * 512, row[j] + at, there ? 16 : 0);
-                if (t == 0) cp_async16(ring + fs * STREAM_SLOT + 2048 + g * 16, exps + fc * MX_TILE_BYTES);
+                if (t == 0) cp_async16(ring + fs * STREAM_SLOT + 2048 + g * 16, exps + (size_t)fc * MX_TILE_BYTES);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             fc += W;
@@ -707,13 +707,11 @@ static void tile_plan(int M, int N, int K, bool &pair, int &bn, int &S) {
     }
 }
 
-#define MX_MOST_ROWS (0x7fffffff - 512)
 static int mx_check(const MxGemm &a) {
     if (a.out_dtype != FG_F32 && a.out_dtype != FG_BF16) return FG_ERR_BAD_DTYPE;
     if (a.accumulate && a.out_dtype != FG_F32) return FG_ERR_BAD_DTYPE;
     if (a.M < 0 || a.N <= 0 || a.K <= 0 || a.K % MX_BLOCK || a.ldx < 0 || a.ldo < 0 || ((uintptr_t)a.w & 15) || ((uintptr_t)a.sc & 15)) return FG_ERR_BAD_SIZE;
-    // rows of x and of all matrices are counted in 31 bits, up to the end of the last tile
-    if (a.M > MX_MOST_ROWS || (long long)a.N * (a.offsets ? a.experts : 1) > MX_MOST_ROWS) return FG_ERR_BAD_SIZE;
+    if (a.M > MX_MOST || a.K > MX_MOST || (long long)a.N * (a.offsets ? a.experts : 1) > MX_MOST) return FG_ERR_BAD_SIZE;
     return 0;
 }
 

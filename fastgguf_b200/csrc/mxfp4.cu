@@ -96,7 +96,7 @@ mxfp4_quantize_kernel(const T *x, long long ldx, long long x_stride, uint8_t *__
 extern "C" int fg_mxfp4_quantize(const void *x, int dtype, long long ldx, long long x_stride, void *data, void *scales, int mats, int R, int K,
                                  cudaStream_t stream) {
     if (dtype != FG_F32 && dtype != FG_BF16) return FG_ERR_BAD_DTYPE;
-    if (mats < 0 || R < 0 || K <= 0 || K % MX_BLOCK || ldx < 0 || ((uintptr_t)data & 15) || ((uintptr_t)scales & 15)) return FG_ERR_BAD_SIZE;
+    if (mats < 0 || R < 0 || R > MX_MOST || K <= 0 || K > MX_MOST || K % MX_BLOCK || ldx < 0 || ((uintptr_t)data & 15) || ((uintptr_t)scales & 15)) return FG_ERR_BAD_SIZE;
     if (mats == 0 || R == 0) return 0;
     const int tiles_r = mx_tiles(R);
     if ((long long)tiles_r * mats > 65535) return FG_ERR_BAD_SIZE;
@@ -179,7 +179,7 @@ mxfp4_rows_kernel(const uint8_t *data, const uint8_t *scales, const int *rows, T
 extern "C" int fg_mxfp4_rows(const void *data, const void *scales, const int *rows, void *out, int out_dtype, long long ldo, int n, int R, int K,
                              float scale, cudaStream_t stream) {
     if (out_dtype != FG_F32 && out_dtype != FG_BF16) return FG_ERR_BAD_DTYPE;
-    if (n < 0 || R < 0 || K <= 0 || K % MX_BLOCK || ldo < K || (!rows && n > R) || ((uintptr_t)data & 3)) return FG_ERR_BAD_SIZE;
+    if (n < 0 || R < 0 || K <= 0 || K > MX_MOST || K % MX_BLOCK || ldo < K || (!rows && n > R) || ((uintptr_t)data & 3)) return FG_ERR_BAD_SIZE;
     const unsigned per_row = K / 8;
     const int most = (int)(0x7fffffffu / per_row);                   // rows of a launch: pieces are counted in 31 bits
     const unsigned long long over = ~0ull / per_row + 1;

@@ -11,6 +11,7 @@
 
 #define MX_BLOCK 32
 #define MX_TILE_BYTES 512      // exponents of 128 rows x 128 numbers
+#define MX_MOST (0x7fffffff - 512)      // rows (of x, of all matrices of a stack) and numbers of a row are counted in 31 bits, up to the end of the last tile
 
 __host__ __device__ __forceinline__ int mx_tiles(int n) { return (n + 127) / 128; }
 __host__ __device__ __forceinline__ size_t mx_scale_bytes(int rows, int K) { return (size_t)mx_tiles(rows) * mx_tiles(K) * MX_TILE_BYTES; }

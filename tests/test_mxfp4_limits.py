@@ -129,3 +129,41 @@ def test_an_output_is_the_weight_of_the_next_contraction(n, rows):
         for g, y in zip(recorded, want):
             assert all((p is None and q is None) or torch.equal(p, q) for p, q in zip(g, y))
     ops.raise_on_device_error("chains")
+
+
+# ------------------------------------------------------------------------------ long rows
+def test_launchers_refuse_rows_whose_end_passes_31_bits():
+    """Before they touch the device or the memory (the addresses here are none)."""
+    from ctypes import c_void_p
+    L, refused, at = ops.lib("mx"), 10002, c_void_p(1 << 20)                      # (FG_ERR_BAD_SIZE)
+    for k in (2 ** 31 - 32, 2 ** 31 - 128, 2 ** 31 - 480):
+        assert L.fg_gemm_mxfp4(at, k, at, at, at, 1, 4, 0, 1, 4, k, None) == refused
+        assert L.fg_gemm_mxfp4_both(at, at, at, at, at, 1, 4, 0, 1, 4, k, None) == refused
+        assert L.fg_gemm_mxfp4_grouped(at, k, at, at, at, 2, at, 1, 4, 0, 1, 4, k, None) == refused
+        assert L.fg_mxfp4_quantize(at, 0, k, 0, at, at, 1, 1, k, None) == refused
+        assert L.fg_mxfp4_rows(at, at, at, at, 0, k, 1, 1, k, 1.0, None) == refused
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [2 ** 29 + 160, 3 * 2 ** 28 + 96])
+def test_the_end_of_a_long_row(k):
+    """Rows whose exponents take more than 2^31 bytes: numbers behind that place count as they should."""
+    n = 3
+    data, scales = torch.zeros(n, k // 2, dtype=torch.uint8, device="cuda"), torch.zeros(1, (k + 127) // 128, 32, 4, 4, dtype=torch.uint8, device="cuda")
+    tail_data, tail_e = plain.random_matrix(n, 320, _gen(1))
+    first = (k - 320) // 32                                    # the block where the last 320 numbers start
+    data[:, -160:] = tail_data.cuda()
+    for r in range(n):
+        for b in range(10):
+            scales[0, (first + b) // 4, r, 0, (first + b) % 4] = tail_e[r, b]
+    w = Mxfp4(data, scales)
+    x = torch.zeros(1, k, dtype=torch.bfloat16, device="cuda")
+    x[:, -320:] = _rows(1, 320, 2).cuda()
+    x[:, 64:96] = 1.0                                          # (under weights of zero)
+    want, slack = plain.product(x[:, -320:].cpu(), plain.numbers(tail_data, tail_e))
+    plain.check(ops.gemm_mxfp4(x, w, out_dtype=torch.float32), want, slack)
+    q = ops.mxfp4_quantize(x)
+    rounded = plain.rounded(x[:, -320:].cpu())[0]
+    assert torch.equal(ops.mxfp4_rows(q, out_dtype=torch.bfloat16)[:, -320:].double().cpu(), rounded)
+    want, slack = plain.product(rounded, plain.numbers(tail_data, tail_e))
+    plain.check(ops.gemm_mxfp4_both(q, w, out_dtype=torch.float32), want, slack)
