@@ -35,6 +35,7 @@ register_signatures("mx", {
 })
 
 BLOCK = 32
+MOST = 2 ** 31 - 1                               # of the launchers' C integers (their own limits are finer)
 _CODES = {torch.float32: FG_F32, torch.bfloat16: FG_BF16}
 
 
@@ -128,6 +129,12 @@ def _on_one_device(what: str, *tensors) -> int:
     return device
 
 
+def _counted(what: str, *sizes: int) -> None:
+    """(a size that passes 31 bits would reach the kernels as another one)"""
+    if max(sizes) > MOST:
+        raise KernelError(f"{what}: sizes go up to {MOST}, got {max(sizes)}")
+
+
 def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
     """x [rows, K] or [X, rows, K], float32 or bfloat16, K a multiple of 32, to MXFP4.
 
@@ -144,6 +151,7 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
         raise KernelError(f"mxfp4_quantize: rows of {k} numbers are not whole blocks of {BLOCK}")
     if x.stride(-1) != 1:
         raise KernelError("mxfp4_quantize: the numbers of a row must be contiguous")
+    _counted("mxfp4_quantize", *x.shape)
     lead = x.shape[:-2]
     q = Mxfp4.__new__(Mxfp4)                     # (as its constructor would leave it)
     q.rows, q.k = rows, k
@@ -164,6 +172,7 @@ def mxfp4_rows(w: Mxfp4, rows: Optional[torch.Tensor] = None, *, scale: float = 
     if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous()):
         raise KernelError(f"mxfp4_rows: rows must be a contiguous int32 vector, got {rows.dtype} {tuple(rows.shape)}")
     n = w.rows if rows is None else rows.numel()
+    _counted("mxfp4_rows", n, w.rows, w.k)
     if out is None:
         out = w.data.new_empty((n, w.k), dtype=out_dtype or torch.float32)
     elif out.shape != (n, w.k) or out.stride(1) != 1 or (n > 1 and out.stride(0) < w.k) or (out_dtype is not None and out.dtype != out_dtype):
@@ -176,7 +185,8 @@ def mxfp4_rows(w: Mxfp4, rows: Optional[torch.Tensor] = None, *, scale: float = 
     return out
 
 
-def _output(what: str, M: int, N: int, like: torch.Tensor, out, out_dtype, accumulate: bool) -> tuple:
+def _output(what: str, M: int, N: int, K: int, like: torch.Tensor, out, out_dtype, accumulate: bool) -> tuple:
+    _counted(what, M, N, K)
     if out is None:
         if accumulate:
             raise KernelError(f"{what}: accumulate needs the tensor to accumulate into")
@@ -210,7 +220,7 @@ def gemm_mxfp4(x: torch.Tensor, w: Mxfp4, *, out: Optional[torch.Tensor] = None,
         raise KernelError("gemm_mxfp4: w is one matrix, not a stack (see gemm_mxfp4_grouped)")
     _activations("gemm_mxfp4", x, w.k)
     M = x.shape[0]
-    out, code = _output("gemm_mxfp4", M, w.rows, data, out, out_dtype, accumulate)
+    out, code = _output("gemm_mxfp4", M, w.rows, w.k, data, out, out_dtype, accumulate)
     _launch("gemm_mxfp4", device, x.data_ptr(), x.stride(0), data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code, out.stride(0),
             accumulate, M, w.rows, w.k)
     return out
@@ -225,7 +235,7 @@ def gemm_mxfp4_both(x: Mxfp4, w: Mxfp4, *, out: Optional[torch.Tensor] = None, o
     if x.k != w.k:
         raise KernelError(f"gemm_mxfp4_both: x is {x.shape} but w is {w.shape}")
     M = x.rows
-    out, code = _output("gemm_mxfp4_both", M, w.rows, w.data, out, out_dtype, accumulate)
+    out, code = _output("gemm_mxfp4_both", M, w.rows, w.k, w.data, out, out_dtype, accumulate)
     _launch("gemm_mxfp4_both", device, x.data.data_ptr(), x.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), code,
             out.stride(0), accumulate, M, w.rows, w.k)
     return out
@@ -245,7 +255,7 @@ def gemm_mxfp4_grouped(x: torch.Tensor, w: Mxfp4, offsets: torch.Tensor, *, out:
         raise KernelError(f"gemm_mxfp4_grouped: offsets must be contiguous int32 [{X + 1}], got {offsets.dtype} {tuple(offsets.shape)}")
     _activations("gemm_mxfp4_grouped", x, w.k)
     M = x.shape[0]
-    out, code = _output("gemm_mxfp4_grouped", M, w.rows, w.data, out, out_dtype, accumulate)
+    out, code = _output("gemm_mxfp4_grouped", M, w.rows, w.k, w.data, out, out_dtype, accumulate)
     _launch("gemm_mxfp4_grouped", device, x.data_ptr(), x.stride(0), w.data.data_ptr(), w.scales.data_ptr(), offsets.data_ptr(), X, out.data_ptr(),
             code, out.stride(0), accumulate, M, w.rows, w.k)
     return out

@@ -167,3 +167,37 @@ def test_the_end_of_a_long_row(k):
     assert torch.equal(ops.mxfp4_rows(q, out_dtype=torch.bfloat16)[:, -320:].double().cpu(), rounded)
     want, slack = plain.product(rounded, plain.numbers(tail_data, tail_e))
     plain.check(ops.gemm_mxfp4_both(q, w, out_dtype=torch.float32), want, slack)
+
+
+# ------------------------------------------------------------------------------ sizes beyond 31 bits
+def test_sizes_beyond_31_bits_are_refused_not_cut(monkeypatch):
+    from fastgguf_b200.ops import KernelError, mxfp4
+    monkeypatch.setattr(mxfp4, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(mxfp4, "_on_one_device", lambda *t: 0)
+    monkeypatch.setattr(mxfp4, "_launch", lambda *a: pytest.fail("a refused call reached a kernel"))
+
+    def tensor(*shape, dtype=torch.uint8):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    def matrix(rows, k, lead=()):
+        return Mxfp4(tensor(*lead, rows, k // 2), tensor(*lead, (rows + 127) // 128, (k + 127) // 128, 32, 4, 4))
+
+    many = 2 ** 32 + 32                                    # would reach a kernel as 32
+    small = matrix(4, 64)
+    calls = [
+        lambda: ops.mxfp4_quantize(tensor(many, 64, dtype=torch.float32)),
+        lambda: ops.mxfp4_quantize(tensor(2, many, dtype=torch.bfloat16)),
+        lambda: ops.mxfp4_quantize(tensor(many, 2, 64, dtype=torch.bfloat16)),
+        lambda: ops.mxfp4_rows(matrix(many, 64)),
+        lambda: ops.mxfp4_rows(matrix(4, many)),
+        lambda: ops.mxfp4_rows(small, tensor(many, dtype=torch.int32)),
+        lambda: ops.gemm_mxfp4(tensor(many, 64, dtype=torch.bfloat16), small),
+        lambda: ops.gemm_mxfp4(tensor(2, 64, dtype=torch.bfloat16), matrix(many, 64)),
+        lambda: ops.gemm_mxfp4(tensor(2, many, dtype=torch.bfloat16), matrix(4, many)),
+        lambda: ops.gemm_mxfp4_both(matrix(many, 64), small),
+        lambda: ops.gemm_mxfp4_both(matrix(2, many), matrix(4, many)),
+        lambda: ops.gemm_mxfp4_grouped(tensor(many, 64, dtype=torch.bfloat16), matrix(4, 64, (3,)), tensor(4, dtype=torch.int32)),
+    ]
+    for call in calls:
+        with pytest.raises(KernelError, match="sizes go up to"):
+            call()
