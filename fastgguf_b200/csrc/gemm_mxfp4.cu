@@ -734,8 +734,16 @@ extern "C" int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, co
     if (form == 2) return launch_tiles<false>(a, bn, splits, stream);
     if (form == 3) return launch_tiles<true>(a, bn, 1, stream);
     if (M <= 8) return launch_stream<1>(a, 1, 1, stream);
-    if (M > 65535 * 16) return FG_ERR_BAD_SIZE;
-    return launch_stream<2>(a, (M + 15) / 16, (M + 15) / 16, stream);
+    // (as many tiles of 16 rows a launch as a grid's second dimension takes)
+    for (long long m0 = 0; m0 < M; m0 += 65535 * 16) {
+        MxGemm part = a;
+        part.x += m0 * ldx;
+        part.out = (char *)out + m0 * ldo * (out_dtype == FG_F32 ? 4 : 2);
+        part.M = M - m0 < 65535 * 16 ? (int)(M - m0) : 65535 * 16;
+        const int tiles = (part.M + 15) / 16, rc = launch_stream<2>(part, tiles, tiles, stream);
+        if (rc) return rc;
+    }
+    return 0;
 }
 extern "C" int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
                              int M, int N, int K, cudaStream_t stream) {

@@ -201,3 +201,27 @@ def test_sizes_beyond_31_bits_are_refused_not_cut(monkeypatch):
     for call in calls:
         with pytest.raises(KernelError, match="sizes go up to"):
             call()
+
+
+# ------------------------------------------------------------------------------ many rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("stride", [33, 0])
+@pytest.mark.parametrize("m", [65535 * 16, 65535 * 16 + 1, 2 * 65535 * 16 + 37])
+def test_more_rows_than_a_grid_takes_where_tma_cannot_address_them(m, stride):
+    n, k = 5, 32
+    data, e = plain.random_matrix(n, k, _gen(1))
+    w, numbers = Mxfp4.from_exponents(data.cuda(), e.cuda()), plain.numbers(data, e)
+    if stride:
+        x = torch.randn(m, stride, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").bfloat16()[:, :k]
+    else:
+        x = _rows(1, k, 3).cuda().expand(m, k)
+    want, slack = plain.product(x.cpu(), numbers)
+    for dtype in (torch.bfloat16, torch.float32):
+        room = torch.full((m + 2, n + 1), 7.0, dtype=dtype, device="cuda")
+        ops.gemm_mxfp4(x, w, out=room[1:m + 1, :n])
+        plain.check(room[1:m + 1, :n], want, slack)
+        room[1:m + 1, :n] = 7.0
+        assert (room == 7.0).all()
+    total = torch.ones(m, n, device="cuda")
+    ops.gemm_mxfp4(x, w, out=total, accumulate=True)
+    plain.check(total, want + 1.0, slack + 2.0 ** -24)
