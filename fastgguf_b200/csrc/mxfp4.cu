@@ -98,14 +98,22 @@ extern "C" int fg_mxfp4_quantize(const void *x, int dtype, long long ldx, long l
     if (dtype != FG_F32 && dtype != FG_BF16) return FG_ERR_BAD_DTYPE;
     if (mats < 0 || R < 0 || R > MX_MOST || K <= 0 || K > MX_MOST || K % MX_BLOCK || ldx < 0 || ((uintptr_t)data & 15) || ((uintptr_t)scales & 15)) return FG_ERR_BAD_SIZE;
     if (mats == 0 || R == 0) return 0;
-    const int tiles_r = mx_tiles(R);
-    if ((long long)tiles_r * mats > 65535) return FG_ERR_BAD_SIZE;
+    // A launch takes up to 65,535 tiles of 128 rows: whole matrices, or a share of one matrix's rows.
+    const int most = 65535, rows = R < most * 128 ? R : most * 128, together = rows < R ? 1 : most / mx_tiles(R);
     const int V = dtype == FG_F32 ? 8 : 16;
     const int vec = (uintptr_t)x % 32 == 0 && ldx % V == 0 && x_stride % V == 0;
-    dim3 grid(mx_tiles(K), tiles_r * mats);
-    if (dtype == FG_F32)
-        return mx_launch(mxfp4_quantize_kernel<float>, grid, 256, 0, dim3(1, 1, 1), stream, (const float *)x, ldx, x_stride, (uint8_t *)data, (uint8_t *)scales, R, K, tiles_r, vec);
-    return mx_launch(mxfp4_quantize_kernel<bf16>, grid, 256, 0, dim3(1, 1, 1), stream, (const bf16 *)x, ldx, x_stride, (uint8_t *)data, (uint8_t *)scales, R, K, tiles_r, vec);
+    for (long long m = 0; m < mats; m += together)
+        for (long long r = 0; r < R; r += rows) {
+            const int n = mats - m < together ? (int)(mats - m) : together, nr = R - r < rows ? (int)(R - r) : rows;
+            const long long at = m * x_stride + r * ldx;
+            uint8_t *d = (uint8_t *)data + ((size_t)m * R + r) * (K / 2), *s = (uint8_t *)scales + m * mx_scale_bytes(R, K) + mx_scale_bytes((int)r, K);
+            const dim3 grid(mx_tiles(K), mx_tiles(nr) * n);
+            const int rc = dtype == FG_F32
+                ? mx_launch(mxfp4_quantize_kernel<float>, grid, 256, 0, dim3(1, 1, 1), stream, (const float *)x + at, ldx, x_stride, d, s, nr, K, mx_tiles(nr), vec)
+                : mx_launch(mxfp4_quantize_kernel<bf16>, grid, 256, 0, dim3(1, 1, 1), stream, (const bf16 *)x + at, ldx, x_stride, d, s, nr, K, mx_tiles(nr), vec);
+            if (rc) return rc;
+        }
+    return 0;
 }
 
 // ---------------------------------------------------------------------------- rows

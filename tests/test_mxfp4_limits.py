@@ -225,3 +225,23 @@ def test_more_rows_than_a_grid_takes_where_tma_cannot_address_them(m, stride):
     total = torch.ones(m, n, device="cuda")
     ops.gemm_mxfp4(x, w, out=total, accumulate=True)
     plain.check(total, want + 1.0, slack + 2.0 ** -24)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lead,rows,k", [((65536,), 1, 32), ((33000,), 129, 160), ((), 65535 * 128 + 1, 32), ((), 65537 * 128, 64)])
+def test_quantising_more_tiles_than_a_grids_second_dimension(dtype, lead, rows, k):
+    x = torch.randn(*lead, rows, k, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    q = ops.mxfp4_quantize(x)
+    if lead:
+        for i in (0, 1, 32767, lead[0] - 1):
+            want, e = plain.rounded(x[i])
+            assert torch.equal(q[i].exponents().cpu(), e) and torch.equal(plain.of(q[i]), want)
+        some = torch.randint(0, lead[0], (200,), generator=_gen(2)).tolist()
+        data, e = zip(*((q[i].data, q[i].exponents()) for i in some))
+        want, want_e = plain.rounded(x[some].reshape(-1, k))
+        assert torch.equal(torch.cat(e).cpu(), want_e) and torch.equal(plain.numbers(torch.cat(data), torch.cat(e)), want)
+    else:
+        back = ops.mxfp4_rows(q)
+        for at in (0, 127, 4194304, rows - 300):
+            assert torch.equal(back[at:at + 300].double().cpu(), plain.rounded(x[at:at + 300])[0])
