@@ -129,10 +129,9 @@ def _on_one_device(what: str, *tensors) -> int:
     return device
 
 
-def _counted(what: str, *sizes: int) -> None:
+def _too_large(what: str, *sizes: int) -> None:
     """(a size that passes 31 bits would reach the kernels as another one)"""
-    if max(sizes) > MOST:
-        raise KernelError(f"{what}: sizes go up to {MOST}, got {max(sizes)}")
+    raise KernelError(f"{what}: sizes go up to {MOST}, got {max(sizes)}")
 
 
 def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
@@ -151,8 +150,9 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
         raise KernelError(f"mxfp4_quantize: rows of {k} numbers are not whole blocks of {BLOCK}")
     if x.stride(-1) != 1:
         raise KernelError("mxfp4_quantize: the numbers of a row must be contiguous")
-    _counted("mxfp4_quantize", *x.shape)
     lead = x.shape[:-2]
+    if rows > MOST or k > MOST or (lead and lead[0] > MOST):
+        _too_large("mxfp4_quantize", *x.shape)
     q = Mxfp4.__new__(Mxfp4)                     # (as its constructor would leave it)
     q.rows, q.k = rows, k
     q.data = data = x.new_empty((*lead, rows, k // 2), dtype=torch.uint8)
@@ -172,7 +172,8 @@ def mxfp4_rows(w: Mxfp4, rows: Optional[torch.Tensor] = None, *, scale: float = 
     if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous()):
         raise KernelError(f"mxfp4_rows: rows must be a contiguous int32 vector, got {rows.dtype} {tuple(rows.shape)}")
     n = w.rows if rows is None else rows.numel()
-    _counted("mxfp4_rows", n, w.rows, w.k)
+    if n > MOST or w.rows > MOST or w.k > MOST:
+        _too_large("mxfp4_rows", n, w.rows, w.k)
     if out is None:
         out = w.data.new_empty((n, w.k), dtype=out_dtype or torch.float32)
     elif out.shape != (n, w.k) or out.stride(1) != 1 or (n > 1 and out.stride(0) < w.k) or (out_dtype is not None and out.dtype != out_dtype):
@@ -186,7 +187,8 @@ def mxfp4_rows(w: Mxfp4, rows: Optional[torch.Tensor] = None, *, scale: float = 
 
 
 def _output(what: str, M: int, N: int, K: int, like: torch.Tensor, out, out_dtype, accumulate: bool) -> tuple:
-    _counted(what, M, N, K)
+    if M > MOST or N > MOST or K > MOST:
+        _too_large(what, M, N, K)
     if out is None:
         if accumulate:
             raise KernelError(f"{what}: accumulate needs the tensor to accumulate into")
