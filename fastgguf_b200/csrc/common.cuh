@@ -136,15 +136,20 @@ __device__ __forceinline__ void pdl_launch_dependents_small_step(unsigned rows) 
 }
 
 #include <cstdlib>
-// Function attributes (the dynamic shared memory limit) belong to a kernel on ONE device: a launcher sets them the
-// first time it runs on each device.  True once per device for the call site that owns `s`.
-struct FgPerDevice { bool done[64]; };
+#include "set_up.h"
+// Function attributes (the dynamic shared memory limit) belong to a kernel on ONE device: a launcher sets them with `set_up` in its first call on
+// each device.  0, or the error.
+template <typename F>
+static inline int fg_set_up(FgPerDevice &s, F set_up) {
+    int dev = 0, code = (int)cudaGetDevice(&dev);
+    if (!code) code = fg_set_up_on(s, dev, set_up);
+    if (code) cudaGetLastError();
+    return code;
+}
 static inline bool fg_needs_setup(FgPerDevice &s) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (s.done[dev]) return false;
-    s.done[dev] = true;
-    return true;
+    return !s.done[dev].exchange(true);
 }
 
 static inline bool fg_pdl_enabled() {

@@ -257,45 +257,53 @@ struct MxStreamForm {
     static constexpr int groups = STREAM_ALL / W, fixed = STREAM_ALL * (STREAM_RING(NT) * STREAM_SLOT + 8 * NT * STREAM_ROWS * 4), room_bytes = fixed + 65536;
     static int setup() {
         static FgPerDevice configured;
-        return fg_needs_setup(configured) ? (int)cudaFuncSetAttribute(mxfp4_stream_kernel<NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, room_bytes) : 0;
+        return fg_set_up(configured, [] { return cudaFuncSetAttribute(mxfp4_stream_kernel<NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, room_bytes); });
     }
-    static int room(int S) {                                         // CTAs (a cluster of S each) that fit at once
+    static int width(int S, int busy, int units, int &gx) {          // CTAs (a cluster of S each) along the units, as many as fit at once
         static MxClusters known;
-        return mx_clusters(known, mxfp4_stream_kernel<NT, W>, STREAM_THREADS, room_bytes, S);
-    }
-    static int width(int S, int busy, int units) {                   // CTAs along the units
-        const int most = (units + groups - 1) / groups, gx = room(S) / busy;
-        return gx < 1 ? 1 : gx > most ? most : gx;
+        int fit = 0;
+        const int rc = mx_clusters(known, mxfp4_stream_kernel<NT, W>, STREAM_THREADS, room_bytes, S, fit), most = (units + groups - 1) / groups;
+        gx = fit / busy < 1 ? 1 : fit / busy > most ? most : fit / busy;
+        return rc;
     }
     // The split of K that finishes first, in us: rounds of units times a warp's chunks and the sums behind them.  Fitted to us | us with groups of eight | four
     // warps, eight rows: 28,672 x 4,096: 23.5 | 22.6; 16,384 x 2,048: 9.6 | 8.9; 4,096 x 14,336: 16.6 | 13.9; 8,192 x 2,048: 6.0 | 6.6 (it splits K);
     // 2,048 x 8,192: 7.4 | 9.3; one row of 128,256 x 2,048: 42.5 | 35.1 (sums of half as many warps, half as often).
-    static double plan(int units, int tiles_k, int busy, int &S) {
-        double best = 1e30;
-        if (setup()) cudaGetLastError();                             // (its launch reports it)
+    static int plan(int units, int tiles_k, int busy, int &S, double &best) {
+        best = 1e30;
+        const int rc = setup();
+        if (rc) return rc;
         for (int s = 1; s <= 8; s *= 2) {
             if (s < 8 && tiles_k > s * STREAM_CHUNKS(NT)) continue;  // until x fits at once
             if (best < 1e30 && tiles_k <= s / 2 * W) break;          // each warp keeps a chunk
             const int chunks = ((tiles_k + s - 1) / s + W - 1) / W;
-            const long long lanes = (long long)width(s, busy, units) * groups, rounds = (units + lanes - 1) / lanes;
+            int gx = 1;
+            const int bad = width(s, busy, units, gx);
+            if (bad) return bad;
+            const long long lanes = (long long)gx * groups, rounds = (units + lanes - 1) / lanes;
             const double cost = rounds * (1.1 * chunks + (W == 8 ? 0.55 : 0.2) + (s > 1 ? (W == 8 ? 0.35 : 0.45) * s : 0.0));
             if (cost < best) { best = cost; S = s; }
         }
-        return best;
+        return 0;
     }
-    static int launch(MxGemm a, int y, int busy, int units, int S, cudaStream_t stream) {
-        const int rc = setup(), tiles_k = mx_tiles(a.K);
+    static int launch(MxGemm a, int y, int busy, int units, int S, cudaStream_t stream) {      // (behind plan)
+        const int tiles_k = mx_tiles(a.K);
+        int gx = 1;
+        const int rc = width(S, busy, units, gx);
         if (rc) return rc;
         a.chunks_per_split = (tiles_k + S - 1) / S;
         const int staged = a.chunks_per_split < STREAM_CHUNKS(NT) ? a.chunks_per_split : STREAM_CHUNKS(NT);
-        return mx_launch(mxfp4_stream_kernel<NT, W>, dim3(width(S, busy, units), y, S), STREAM_THREADS, fixed + staged * NT * 2048, dim3(1, 1, S), stream, a, units);
+        return mx_launch(mxfp4_stream_kernel<NT, W>, dim3(gx, y, S), STREAM_THREADS, fixed + staged * NT * 2048, dim3(1, 1, S), stream, a, units);
     }
 };
 template <int NT>
 static int launch_stream(const MxGemm &a, int y, int busy /* of the y, that have rows */, cudaStream_t stream) {
     const int units = 4 * mx_tiles(a.N), tiles_k = mx_tiles(a.K);
     int s8 = 1, s4 = 1;
-    const double eight = MxStreamForm<NT, 8>::plan(units, tiles_k, busy, s8), four = MxStreamForm<NT, 4>::plan(units, tiles_k, busy, s4);
+    double eight, four;
+    int rc = MxStreamForm<NT, 8>::plan(units, tiles_k, busy, s8, eight);
+    if (!rc) rc = MxStreamForm<NT, 4>::plan(units, tiles_k, busy, s4, four);
+    if (rc) return rc;
     return four < eight ? MxStreamForm<NT, 4>::launch(a, y, busy, units, s4, stream) : MxStreamForm<NT, 8>::launch(a, y, busy, units, s8, stream);
 }
 
@@ -646,7 +654,7 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
 template <bool PAIR>
 static int tile_setup() {
     static FgPerDevice configured;
-    return fg_needs_setup(configured) ? (int)cudaFuncSetAttribute(mxfp4_tile_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM) : 0;
+    return fg_set_up(configured, [] { return cudaFuncSetAttribute(mxfp4_tile_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM); });
 }
 
 template <bool PAIR>
@@ -682,10 +690,13 @@ static bool tile_ok(const MxGemm &g) { return g.x_vec && g.ldx >= g.K; }
 // measured at both ends (pairs: 820 cycles at 128 tokens, 1,350 at 256; single CTAs, bound by the bytes an SM receives: 950 and 1,690).  Half of a
 // step counts whole rounds of tiles over the SMs, half the tiles alone: at the power limit the clock rises while SMs are idle (2,048 x 14,336 x 4,096 in
 // seven rounds of 256 tokens takes 161 to 180 us, in the ten of 160 tokens, 7 % fewer by rounds, 192).
-static void tile_plan(int M, int N, int K, bool &pair, int &bn, int &S) {
+static int tile_plan(int M, int N, int K, bool &pair, int &bn, int &S) {
     static MxClusters known;
     const int tiles_k = mx_tiles(K), n_sm = mx_sm_count();
-    if (tile_setup<false>()) cudaGetLastError();                     // (its launch reports it)
+    int fit[9];
+    int rc = tile_setup<false>();
+    for (int s = 1; s <= 8 && !rc; s++) rc = mx_clusters(known, mxfp4_tile_kernel<false>, TILE_THREADS, TILE_SMEM, s, fit[s]);
+    if (rc) return rc;
     double best = 1e30;
     for (int p = 0; p < 2; p++) {
         const int rows = p ? 2 * TILE_ROWS : TILE_ROWS, tiles_n = (N + rows - 1) / rows, units = p ? n_sm / 2 : n_sm;
@@ -694,7 +705,7 @@ static void tile_plan(int M, int N, int K, bool &pair, int &bn, int &S) {
             if (b > step && b - step >= M) break;                    // wider than the rows there are
             const long long tiles = (long long)((M + b - 1) / b) * tiles_n;
             for (int s = 1; s <= (p ? 1 : 8); s++) {
-                if (s > 1 && tiles > mx_clusters(known, mxfp4_tile_kernel<false>, TILE_THREADS, TILE_SMEM, s)) continue;
+                if (s > 1 && tiles > fit[s]) continue;
                 const int kb = (tiles_k + s - 1) / s;
                 const double mma = p ? 300 + 4.1 * b : 210 + 5.8 * b, stage = mma > TILE_UNPACK ? mma : TILE_UNPACK;
                 const double tile = kb * stage + 2500 + 4.0 * b + (s > 1 ? 2500 + 8.0 * b : 0);
@@ -705,6 +716,7 @@ static void tile_plan(int M, int N, int K, bool &pair, int &bn, int &S) {
             }
         }
     }
+    return 0;
 }
 
 static int mx_check(const MxGemm &a) {
@@ -727,7 +739,10 @@ extern "C" int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, co
     if (form == 0) {
         bool pair = false;
         form = M > 8 && tile_ok(a) ? 2 : 1;
-        if (form == 2) tile_plan(M, N, K, pair, bn, splits);
+        if (form == 2) {
+            const int rc = tile_plan(M, N, K, pair, bn, splits);
+            if (rc) return rc;
+        }
         if (pair) form = 3;
     } else if (form < 1 || form > 3 || (form > 1 && (!tile_ok(a) || bn < 16 || bn > 256 || bn % 16 || splits < 1 || splits > 8 || (form == 3 && (splits > 1 || bn % 32)))))
         return FG_ERR_BAD_SIZE;

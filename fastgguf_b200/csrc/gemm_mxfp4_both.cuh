@@ -185,7 +185,7 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
 
 static int both_setup() {
     static FgPerDevice configured;
-    return fg_needs_setup(configured) ? (int)cudaFuncSetAttribute(mxfp4_both_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BOTH_SMEM) : 0;
+    return fg_set_up(configured, [] { return cudaFuncSetAttribute(mxfp4_both_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BOTH_SMEM); });
 }
 
 static int launch_both(MxBoth a, const void *x, int bn, int S, cudaStream_t stream) {
@@ -216,9 +216,12 @@ static int launch_both(MxBoth a, const void *x, int bn, int S, cudaStream_t stre
 
 // The tile's width and the split of K that finish first: rounds of tiles over the SMs times what a tile takes, in SM cycles.  Tiles of
 // more than one start at multiples of 128 tokens, where tiles of exponents do.
-static void both_plan(int M, int N, int K, int &bn, int &S) {
+static int both_plan(int M, int N, int K, int &bn, int &S) {
     static MxClusters known;
-    if (both_setup()) cudaGetLastError();                            // (its launch reports it)
+    int fit[9];
+    int rc = both_setup();
+    for (int s = 1; s <= 8 && !rc; s++) rc = mx_clusters(known, mxfp4_both_kernel, BOTH_THREADS, BOTH_SMEM, s, fit[s]);
+    if (rc) return rc;
     const int n_sm = mx_sm_count(), all_kb = (K + BOTH_K - 1) / BOTH_K, tiles_n = mx_tiles(N), whole = (M + 15) / 16 * 16;
     const int widths[2] = {whole < 256 ? whole : 256, whole < 128 ? whole : 128};
     double best = 1e30;
@@ -226,13 +229,14 @@ static void both_plan(int M, int N, int K, int &bn, int &S) {
         const int b = widths[i];
         const long long tiles = (long long)((M + b - 1) / b) * tiles_n;
         for (int s = 1; s <= 8; s++) {
-            if (s > 1 && tiles > mx_clusters(known, mxfp4_both_kernel, BOTH_THREADS, BOTH_SMEM, s)) continue;
+            if (s > 1 && tiles > fit[s]) continue;
             const int kb = (all_kb + s - 1) / s;
             const double tile = kb * (300 + 1.9 * b) + 2500 + 5.0 * b + (s > 1 ? 1500 + 12.0 * b : 0);
             const double cost = (double)((tiles * s + n_sm - 1) / n_sm) * tile;
             if (cost < best) { best = cost; bn = b; S = s; }
         }
     }
+    return 0;
 }
 
 // x, w and their exponents in the format; bn, splits: 0 by the rule, else (tests, measurements) tokens a tile - a multiple of 128 up to 256, or a multiple of 16
@@ -246,8 +250,10 @@ extern "C" int fg_gemm_mxfp4_both_ext(const void *x, const void *x_scales, const
     if (bad) return bad;
     if (((uintptr_t)x & 15) || ((uintptr_t)x_scales & 15)) return FG_ERR_BAD_SIZE;
     if (M == 0) return 0;
-    if (bn == 0) both_plan(M, N, K, bn, splits);
-    else if (bn < 16 || bn > 256 || bn % 16 || (bn % 128 && bn < M) || splits < 1 || splits > 8) return FG_ERR_BAD_SIZE;
+    if (bn == 0) {
+        const int rc = both_plan(M, N, K, bn, splits);
+        if (rc) return rc;
+    } else if (bn < 16 || bn > 256 || bn % 16 || (bn % 128 && bn < M) || splits < 1 || splits > 8) return FG_ERR_BAD_SIZE;
     return launch_both(a, x, bn, splits, stream);
 }
 extern "C" int fg_gemm_mxfp4_both(const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int out_dtype, long long ldo,

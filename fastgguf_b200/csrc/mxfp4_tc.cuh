@@ -166,12 +166,13 @@ __device__ __forceinline__ float4 ld_dsmem_f32x4(uint32_t local_addr, int rank) 
 typedef CUresult (*MxEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 static inline MxEncodeFn mx_encode_fn() {
-    static MxEncodeFn fn = nullptr;
+    static std::atomic<MxEncodeFn> known;
+    MxEncodeFn fn = known.load(std::memory_order_relaxed);
     if (!fn) {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-            fn = (MxEncodeFn)p;
+            known.store(fn = (MxEncodeFn)p, std::memory_order_relaxed);
     }
     return fn;
 }
@@ -189,33 +190,38 @@ static inline int mx_make_map(CUtensorMap *map, const void *base, bool bf16_numb
                     CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : FG_ERR_TENSORMAP;
 }
-static inline int mx_sm_count() {
-    static int n[64] = {0};
+static inline int mx_device() {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (n[dev] == 0 && (cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n[dev] <= 0)) n[dev] = 148;
-    return n[dev];
+    return cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 ? -1 : dev;      // (-1: nothing is kept for it)
 }
-// How many clusters of S CTAs (along z; S 1: CTAs) of a kernel that takes an SM to itself run at once: clusters stay inside a group of SMs, and the groups' sizes
-// are no multiples of S (of 7 or 8, fewer than 16 fit).  Asked once per device and S.
-struct MxClusters { short n[64][9]; };
-template <typename K>
-static inline int mx_clusters(MxClusters &known, K kernel, int threads, int smem, int S) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    short &n = known.n[dev][S];
+static inline int mx_sm_count() {
+    static std::atomic<int> known[64];
+    const int dev = mx_device();
+    int n = dev < 0 ? 0 : known[dev].load(std::memory_order_relaxed);
     if (n == 0) {
-        int got = 0;
-        if (S > 1) {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(1, 1, S); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
-            cfg.attrs = attr; cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess) { got = 0; cudaGetLastError(); }
-        }
-        n = (short)(got > 0 ? got : mx_sm_count() / S);
+        int at = 0;
+        if (cudaGetDevice(&at) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, at) != cudaSuccess || n <= 0) return 148;
+        if (dev >= 0) known[dev].store(n, std::memory_order_relaxed);
     }
     return n;
+}
+// How many clusters of S CTAs (along z; S 1: CTAs) of a kernel that takes an SM to itself run at once: clusters stay inside a group of SMs, and the groups' sizes
+// are no multiples of S (of 7 or 8, fewer than 16 fit).  Asked once per device and S, once the kernel is set up there.  0, or the error of the question.
+struct MxClusters { std::atomic<short> n[64][9]; };
+template <typename K>
+static inline int mx_clusters(MxClusters &known, K kernel, int threads, int smem, int S, int &fit) {
+    if (S == 1) { fit = mx_sm_count(); return 0; }
+    const int dev = mx_device();
+    fit = dev < 0 ? 0 : known.n[dev][S].load(std::memory_order_relaxed);
+    if (fit > 0) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, 1, S); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = S;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    const int rc = (int)cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg);
+    if (rc) { cudaGetLastError(); return rc; }
+    if (dev >= 0 && fit > 0) known.n[dev][S].store((short)fit, std::memory_order_relaxed);
+    return 0;
 }
