@@ -432,10 +432,7 @@ static int launch_decode_f32(const DecodeF32 &a, int B, int n_splits, cudaStream
     using Z = DfSizes<HD, NW, NH>;
     static_assert(Z::SMEM <= 227 * 1024, "a CTA's shared memory");
     static FgPerDevice configured;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(attn_decode_f32_kernel<HD, NW, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::SMEM);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(configured, attn_decode_f32_kernel<HD, NW, NH>, Z::SMEM)) return e;
     const long long blocks = (long long)n_splits * a.KV * ((a.G + NH - 1) / NH) * B;
     if (blocks > 0x7fffffff) return FG_ERR_BAD_SIZE;
     cudaLaunchConfig_t cfg = {};

@@ -446,10 +446,7 @@ static int launch_latent(const void *q, int ldq, void *out, int ldo, const int *
                          const float *sinks, int n_splits, float *part, cudaStream_t stream) {
     static FgPerDevice setup;
     const size_t smem = latent_smem(R, DR);
-    if (fg_needs_setup(setup)) {
-        cudaError_t e = cudaFuncSetAttribute(latent_decode_kernel<T, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(setup, latent_decode_kernel<T, NG>, 200 * 1024)) return e;
     int code = fg_launch(latent_decode_kernel<T, NG>, dim3((H + LAT_HG - 1) / LAT_HG, M, n_splits), dim3(LAT_WARPS * 32), smem, stream, (const T *)q,
                          ldq, (T *)out, ldo, positions, row_seq, block_table, table_width, (const T *)k_pool, (const T *)v_pool, H, R, DR, page_size,
                          scale, sinks, n_splits, part);
@@ -501,7 +498,7 @@ extern "C" int fg_latent_decode_mma(const void *q, int ldq, void *out, int ldo, 
 #define LM_RUN(NT)                                                                                                                       \
     {                                                                                                                                    \
         static FgPerDevice setup;                                                                                                        \
-        if (fg_needs_setup(setup)) cudaFuncSetAttribute(latent_decode_mma_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024); \
+        if (const int e = fg_allow_shared(setup, latent_decode_mma_kernel<NT>, 224 * 1024)) return e; \
     }                                                                                                                                    \
     code = fg_launch(latent_decode_mma_kernel<NT>, grid, dim3(LM_WARPS * 32), smem, stream, (const bf16 *)q, ldq, (bf16 *)out, ldo, \
                                     positions, row_seq, block_table, table_width, (const bf16 *)k_pool, (const bf16 *)v_pool, H, DR, scale_log2, sinks, \

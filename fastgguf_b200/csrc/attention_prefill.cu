@@ -162,10 +162,7 @@ static int launch_prefill(const void *q, int ldq, void *out, int ldo, const int 
                           int v_share, int out_f32, cudaStream_t stream) {
     constexpr int smem = 2 * PAGE * (HD + HV) * 2;
     static FgPerDevice configured;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(attn_prefill_kernel<HD, HV, PF_WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(configured, attn_prefill_kernel<HD, HV, PF_WARPS>, smem)) return e;
     int G = H / KV, Gc = G < 16 ? G : 16, TQ = PF_WARPS * 16 / Gc;
     dim3 grid((max_new + TQ - 1) / TQ, KV * ((G + Gc - 1) / Gc), n_seq);
     return fg_launch(attn_prefill_kernel<HD, HV, PF_WARPS>, grid, dim3(PF_WARPS * 32), (size_t)smem, stream, (const bf16 *)q, ldq, out, ldo, cu_rows,

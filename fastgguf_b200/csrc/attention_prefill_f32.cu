@@ -679,10 +679,7 @@ static int launch_prefill_f32(const float *q, int ldq, float *out, int ldo, cons
                               const int *block_table, int table_width, const float *k_pool, const float *v_pool, int n_seq,
                               int max_new, int H, int KV, float scale, int window, int skip_few, cudaStream_t stream) {
     static FgPerDevice configured;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(attn_prefill_f32_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Tc<HD>::SMEM);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(configured, attn_prefill_f32_kernel<HD>, F32Tc<HD>::SMEM)) return e;
     const int G = H / KV, Gc = G < 16 ? G : 16, TQ = ROWS / Gc;
     const long long blocks = (long long)KV * ((G + Gc - 1) / Gc) * ((max_new + TQ - 1) / TQ);
     if (blocks > 0x7fffffff) return FG_ERR_BAD_SIZE;

@@ -439,10 +439,7 @@ extern "C" int fg_qkv_prepare_step(const float *proj, int ld, const float *bias,
                      ((((uintptr_t)proj) | ((uintptr_t)bias) | ((uintptr_t)q_out) | ((uintptr_t)k_pool) | ((uintptr_t)v_pool)) & 15) == 0;
 #define PREP_RUN(T, VEC) do { \
         static FgPerDevice setup; \
-        if (smem > 48 * 1024 && fg_needs_setup(setup)) { \
-            cudaError_t e = cudaFuncSetAttribute(qkv_prepare_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); \
-            if (e != cudaSuccess) return (int)e; \
-        } \
+        if (const int e = smem > 48 * 1024 ? fg_allow_shared(setup, qkv_prepare_kernel<T, VEC>, 200 * 1024) : 0) return e; \
         return fg_launch(qkv_prepare_kernel<T, VEC>, dim3(M), dim3(threads), smem, stream, proj, ld, bias, conv_w, taps, conv_state, qn_w, kn_w, \
                          eps, cos_t, sin_t, tbl_half, rot_dims, positions, row_seq, cu_rows, slots, block_table, table_width, (T *)q_out, \
                          ldq, (T *)k_pool, (T *)v_pool, H, KV, VH, hd, hdv, page_size, norm_per_head, rot_halves, v_from_k, early); } while (0)

@@ -146,10 +146,10 @@ static inline int fg_set_up(FgPerDevice &s, F set_up) {
     if (code) cudaGetLastError();
     return code;
 }
-static inline bool fg_needs_setup(FgPerDevice &s) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    return !s.done[dev].exchange(true);
+// the common one: up to `bytes` of dynamic shared memory
+template <typename K>
+static inline int fg_allow_shared(FgPerDevice &s, K kernel, int bytes) {
+    return fg_set_up(s, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
 }
 
 static inline bool fg_pdl_enabled() {

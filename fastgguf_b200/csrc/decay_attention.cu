@@ -404,11 +404,11 @@ static int decay_chunked(bf16 *proj, int ld, float *out, int ldo, const int *cu_
                          float *U, bf16 *P, int n_seq, int n_chunks, int H, cudaStream_t stream) {
     constexpr int smem_state = (3 * DC * DK + DC * DV) * 2, smem_out = (DC * DK + DC * 64 + 3 * DK * 64) * 2;
     static FgPerDevice setup;
-    if (fg_needs_setup(setup)) {
-        cudaError_t e = cudaFuncSetAttribute(decay_state_kernel<DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_state);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(decay_out_kernel<DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_out);
-        if (e != cudaSuccess) return (int)e;
-    }
+    const int rc = fg_set_up(setup, [&] {
+        const cudaError_t e = cudaFuncSetAttribute(decay_state_kernel<DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_state);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(decay_out_kernel<DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_out);
+    });
+    if (rc) return rc;
     const int *chunk_row = plan, *chunk_len = plan + n_chunks;
     int code = fg_retention_plan(cu_rows, n_seq, n_chunks, DC, plan, stream);
     if (code) return code;

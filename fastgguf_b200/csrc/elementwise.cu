@@ -636,10 +636,7 @@ extern "C" int fg_pair_combine(const float *a, const float *b, const float *w_a,
         const int per = (E / 4 + threads - 1) / threads;
         const size_t smem = w_a || w_b ? (size_t)E * 2 * sizeof(float) : 0;
         static FgPerDevice configured;
-        if (per > 4 && fg_needs_setup(configured)) {
-            cudaError_t e = cudaFuncSetAttribute(pair_combine_regs_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, 8192 * 2 * (int)sizeof(float));
-            if (e != cudaSuccess) return (int)e;
-        }
+        if (const int e = per > 4 ? fg_allow_shared(configured, pair_combine_regs_kernel<8>, 8192 * 2 * (int)sizeof(float)) : 0) return e;
 #define PC_REGS(PER) fg_launch(pair_combine_regs_kernel<PER>, dim3(M), dim3(threads), smem, stream, a, b, w_a, w_b, scale_a, scale_b, eps, out, E, accumulate)
         return per <= 1 ? PC_REGS(1) : per <= 2 ? PC_REGS(2) : per <= 4 ? PC_REGS(4) : PC_REGS(8);
 #undef PC_REGS

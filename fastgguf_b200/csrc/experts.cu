@@ -547,10 +547,7 @@ template <typename T, int KIND>
 static int moe_grouped_launch(const void *A, int lda, const void *W, void *out, int ldo, const int *offsets, const int *order,
                               const float *pair_weight, int X, int top, int N, int K, float limit, float alpha, cudaStream_t stream) {
     static FgPerDevice setup;
-    if (fg_needs_setup(setup)) {
-        cudaError_t e = cudaFuncSetAttribute(moe_rows_grouped_kernel<T, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(setup, moe_rows_grouped_kernel<T, KIND>, 96 * 1024)) return e;
     const int per_block = 8 * MR_ROWS_OF(KIND);
     return fg_launch(moe_rows_grouped_kernel<T, KIND>, dim3((N + per_block - 1) / per_block, X), dim3(256), (size_t)MG_SLOTS * K * sizeof(float),
                      stream, (const T *)A, lda, (const T *)W, out, ldo, offsets, order, pair_weight, top, N, K, limit, alpha);

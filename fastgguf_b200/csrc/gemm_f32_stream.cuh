@@ -201,10 +201,7 @@ static int launch_f32_stream(const float *A, int lda, const float *W, int ldw, f
     e = make_map_f32(&tmX, A, M, K, lda, MB);
     if (e) return e;
     static FgPerDevice configured;
-    if (fg_needs_setup(configured)) {
-        cudaError_t ce = cudaFuncSetAttribute(gemm_f32_stream_kernel<MB>, cudaFuncAttributeMaxDynamicSharedMemorySize, FST_RING + 128);
-        if (ce != cudaSuccess) return (int)ce;
-    }
+    if (const int e = fg_allow_shared(configured, gemm_f32_stream_kernel<MB>, FST_RING + 128)) return e;
     return fg_launch(gemm_f32_stream_kernel<MB>, dim3(p.n_tiles < ctas ? p.n_tiles : ctas), dim3(FST_THREADS),
                      (size_t)p.stages * (tile_rows + MB) * FST_KC * 4 + p.part_bytes + 128, stream, tmW, tmX, C, ldc, accumulate, M, N, K, tile_rows,
                      p.n_tiles, p.stages, p.row_groups, p.k_groups);

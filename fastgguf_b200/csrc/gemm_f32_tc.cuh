@@ -540,10 +540,7 @@ template <int BN>
 static int launch_f32_pair(const CUtensorMap &tmP, const CUtensorMap &tmQ, const F32Args &a, cudaStream_t stream) {
     constexpr int smem = 2 * 3 * (BM + BN / 2) * BK * 2 + 1024 + F32_EPI_WARPS * F32_STAGING;
     static FgPerDevice configured;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_f32_pair_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(configured, gemm_f32_pair_kernel<BN>, smem)) return e;
     const int n_pt = (a.M + 2 * BM - 1) / (2 * BM), n_tiles = n_pt * ((a.N + BN - 1) / BN) * a.splits, pairs = sm_count() / 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (n_tiles < pairs ? n_tiles : pairs), 1, 1); cfg.blockDim = dim3(F32_THREADS);

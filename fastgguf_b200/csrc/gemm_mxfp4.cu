@@ -257,7 +257,7 @@ struct MxStreamForm {
     static constexpr int groups = STREAM_ALL / W, fixed = STREAM_ALL * (STREAM_RING(NT) * STREAM_SLOT + 8 * NT * STREAM_ROWS * 4), room_bytes = fixed + 65536;
     static int setup() {
         static FgPerDevice configured;
-        return fg_set_up(configured, [] { return cudaFuncSetAttribute(mxfp4_stream_kernel<NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, room_bytes); });
+        return fg_allow_shared(configured, mxfp4_stream_kernel<NT, W>, room_bytes);
     }
     static int width(int S, int busy, int units, int &gx) {          // CTAs (a cluster of S each) along the units, as many as fit at once
         static MxClusters known;
@@ -654,7 +654,7 @@ mxfp4_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
 template <bool PAIR>
 static int tile_setup() {
     static FgPerDevice configured;
-    return fg_set_up(configured, [] { return cudaFuncSetAttribute(mxfp4_tile_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM); });
+    return fg_allow_shared(configured, mxfp4_tile_kernel<PAIR>, TILE_SMEM);
 }
 
 template <bool PAIR>

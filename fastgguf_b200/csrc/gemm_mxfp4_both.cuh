@@ -185,7 +185,7 @@ mxfp4_both_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant
 
 static int both_setup() {
     static FgPerDevice configured;
-    return fg_set_up(configured, [] { return cudaFuncSetAttribute(mxfp4_both_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BOTH_SMEM); });
+    return fg_allow_shared(configured, mxfp4_both_kernel, BOTH_SMEM);
 }
 
 static int launch_both(MxBoth a, const void *x, int bn, int S, cudaStream_t stream) {

@@ -1238,10 +1238,7 @@ static int launch_decode(const CUtensorMap &tmW, const CUtensorMap &tmX, GemmArg
     const int smem = ring + 1024 + (split ? BN * BM * 4 : 0);
     constexpr int smem_max = MAX_STAGES * stage_bytes + 1024;
     static FgPerDevice configured;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_tc_decode_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_max);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(configured, gemm_tc_decode_kernel<BN>, smem_max)) return e;
     return fg_launch_cluster(gemm_tc_decode_kernel<BN>, grid, dim3(DEC_THREADS(BN)), (size_t)smem, stream, (int)grid.z, tmW, tmX, a);
 }
 
@@ -1249,14 +1246,8 @@ template <int BN, int STAGES, int EPI>
 static int launch_prefill(const CUtensorMap &tmP, const CUtensorMap &tmQ, const GemmArgs &a, cudaStream_t stream, int table_tiles = 0) {
     constexpr int smem = STAGES * (BM + BN) * BK * 2 + 1024 + (EPI == EPI_ADD_F32 ? 4 * EPI_STAGE_BYTES : 0);
     static FgPerDevice configured;
-    static int n_sm = 0;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_tc_prefill_kernel<BN, STAGES, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return (int)e;
-        int dev = 0;
-        cudaGetDevice(&dev);
-        if (cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n_sm <= 0) n_sm = 148;
-    }
+    if (const int e = fg_allow_shared(configured, gemm_tc_prefill_kernel<BN, STAGES, EPI>, smem)) return e;
+    const int n_sm = sm_count();
     int n_pt = (a.M + BM - 1) / BM, n_tiles = n_pt * ((a.N + BN - 1) / BN) * (a.splits > 1 ? a.splits : 1);
     if (a.tiles) n_tiles = table_tiles;                // a grouped contraction: as many tiles as its table has
     dim3 grid(n_tiles < n_sm ? n_tiles : n_sm);
@@ -1264,17 +1255,12 @@ static int launch_prefill(const CUtensorMap &tmP, const CUtensorMap &tmQ, const 
                      n_pt, n_tiles);
 }
 
-static int sm_count();
 template <int BN, int STAGES, int EPI>
 static int launch_prefill_pair(const CUtensorMap &tmP, const CUtensorMap &tmQ, const GemmArgs &a, cudaStream_t stream) {
     constexpr int smem = STAGES * (BM + BN / 2) * BK * 2 + 1024 + (EPI == EPI_ADD_F32 ? PAIR_EPI_WARPS(EPI) * EPI_STAGE_BYTES : 0);
     static FgPerDevice configured;
-    static int n_sm = 0;
-    if (fg_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_tc_prefill_pair_kernel<BN, STAGES, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return (int)e;
-        n_sm = sm_count();
-    }
+    if (const int e = fg_allow_shared(configured, gemm_tc_prefill_pair_kernel<BN, STAGES, EPI>, smem)) return e;
+    const int n_sm = sm_count();
     int n_pt = (a.M + 2 * BM - 1) / (2 * BM), n_tiles = n_pt * ((a.N + BN - 1) / BN);
     int pairs = n_sm / 2;
     // the CTAs of a pair are neighbours along x
@@ -1334,11 +1320,13 @@ extern "C" int fg_gemm_tc_max_ss_tiles(int N) {
 // then uses the plain kernel.
 // streaming multiprocessors of the current device (148 on a B200)
 static int sm_count() {
-    static int n = 0;
+    static std::atomic<int> known;
+    int n = known.load(std::memory_order_relaxed);
     if (!n) {
         int dev = 0;
         cudaGetDevice(&dev);
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+        known.store(n, std::memory_order_relaxed);
     }
     return n;
 }

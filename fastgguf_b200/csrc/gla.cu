@@ -321,11 +321,8 @@ extern "C" int fg_gla(const float *proj, int ld, const float *z, int ldz, const 
     if (smem > 200 * 1024) return FG_ERR_BAD_SIZE;
     if (out_dtype != FG_F32 && out_dtype != FG_BF16) return FG_ERR_BAD_DTYPE;
     const bool wide = out_dtype == FG_F32;
-    if (fg_needs_setup(g_gla_seq_setup[wide ? 0 : 1])) {
-        cudaError_t e = wide ? cudaFuncSetAttribute(gla_seq_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)
-                             : cudaFuncSetAttribute(gla_seq_kernel<bf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = wide ? fg_allow_shared(g_gla_seq_setup[0], gla_seq_kernel<float>, 200 * 1024)
+                           : fg_allow_shared(g_gla_seq_setup[1], gla_seq_kernel<bf16>, 200 * 1024)) return e;
     if (wide)
         return fg_launch(gla_seq_kernel<float>, dim3(n_seq, H), dim3(GLA_THREADS), smem, stream, proj, ld, z, ldz, z_bias, norm_w, (float *)out,
                          ldo, cu_rows, slots, state, H, dk, dv, 1.0f / tau, q_scale, eps);
@@ -349,15 +346,9 @@ extern "C" int fg_gla_chunked(const float *proj, int ld, const float *z, int ldz
     if (!fg_gla_chunked_ok(dk, dv) || H <= 0 || H > 65535 || !(tau > 0.f)) return FG_ERR_BAD_SIZE;
     if (out_dtype != FG_F32 && out_dtype != FG_BF16) return FG_ERR_BAD_DTYPE;
     const bool wide = out_dtype == FG_F32;
-    if (fg_needs_setup(g_gla_state_setup)) {
-        cudaError_t e = cudaFuncSetAttribute(gla_chunk_state_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-        if (e != cudaSuccess) return (int)e;
-    }
-    if (fg_needs_setup(g_gla_out_setup[wide ? 0 : 1])) {
-        cudaError_t e = wide ? cudaFuncSetAttribute(gla_chunk_out_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)
-                             : cudaFuncSetAttribute(gla_chunk_out_kernel<bf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(g_gla_state_setup, gla_chunk_state_kernel, 200 * 1024)) return e;
+    if (const int e = wide ? fg_allow_shared(g_gla_out_setup[0], gla_chunk_out_kernel<float>, 200 * 1024)
+                           : fg_allow_shared(g_gla_out_setup[1], gla_chunk_out_kernel<bf16>, 200 * 1024)) return e;
     int *chunk_row = plan, *chunk_len = plan + n_chunks, *seq_chunk0 = plan + 2 * n_chunks;
     const float inv_tau = 1.0f / tau;
     int code = fg_launch(gla_chunk_plan_kernel, dim3(1), dim3(n_seq >= 256 ? 256 : 32), 0, stream, cu_rows, n_seq, chunk_row, chunk_len, seq_chunk0);

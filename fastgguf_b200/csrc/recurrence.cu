@@ -537,7 +537,7 @@ extern "C" int fg_decay_recurrence(const float *q, int ldq, const float *k, int 
 #define REC_LAUNCH(DELTA, NJ_)                                                                                                            \
     do {                                                                                                                                  \
         static FgPerDevice setup;                                                                                                         \
-        if (fg_needs_setup(setup)) cudaFuncSetAttribute(decay_recurrence_kernel<DELTA, NJ_>, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024); \
+        if (const int e = fg_allow_shared(setup, decay_recurrence_kernel<DELTA, NJ_>, 96 * 1024)) return e; \
         return fg_launch(decay_recurrence_kernel<DELTA, NJ_>, grid, dim3(threads), smem, stream, q, ldq, k, ldk, v, ldv, decay, step, skip, out, \
                                   ldo, cu_rows, slots, state, state_stride, H, Hq, d, dv, R, logR, cols, TC, stride);                      \
     } while (0)

@@ -563,10 +563,7 @@ extern "C" int fg_retention_step(const float *proj, int ld, void *out, int out_d
     if (smem > 200 * 1024) return FG_ERR_BAD_SIZE;
 #define RET_SEQ(TO, SLAB) do { \
         static FgPerDevice setup; \
-        if (fg_needs_setup(setup)) { \
-            cudaError_t e = cudaFuncSetAttribute(retention_seq_kernel<TO, SLAB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); \
-            if (e != cudaSuccess) return (int)e; \
-        } \
+        if (const int e = fg_allow_shared(setup, retention_seq_kernel<TO, SLAB>, 200 * 1024)) return e; \
         return fg_launch(retention_seq_kernel<TO, SLAB>, grid, dim3(RET_THREADS), smem, stream, proj, ld, (TO *)out, ldo, positions, cu_rows, slots, cos_t, \
                          sin_t, decay, state, H, dk, dv, k_scale, eps, opts, slab); } while (0)
     if (slab < dv) {
@@ -615,15 +612,9 @@ extern "C" int fg_retention_chunked(const float *proj, int ld, void *out, int ou
     const bool wide = out_dtype == FG_F32;
     size_t s1 = (size_t)RC * (dk + dv) * 4;
     size_t s3 = ((size_t)2 * RC * (dk + 1) + 2 * (size_t)RC * dv + RC * RC + RC) * 4;
-    if (fg_needs_setup(g_state_setup)) {
-        cudaError_t e = cudaFuncSetAttribute(retention_chunk_state_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-        if (e != cudaSuccess) return (int)e;
-    }
-    if (fg_needs_setup(g_out_setup[wide ? 0 : 1])) {
-        cudaError_t e = wide ? cudaFuncSetAttribute(retention_chunk_out_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)
-                             : cudaFuncSetAttribute(retention_chunk_out_kernel<bf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(g_state_setup, retention_chunk_state_kernel, 200 * 1024)) return e;
+    if (const int e = wide ? fg_allow_shared(g_out_setup[0], retention_chunk_out_kernel<float>, 200 * 1024)
+                           : fg_allow_shared(g_out_setup[1], retention_chunk_out_kernel<bf16>, 200 * 1024)) return e;
     int *chunk_row = plan, *chunk_len = plan + n_chunks;
     // head sizes 64 / 128 with 16-byte aligned rows: the kernels with register tiles
     const bool fast = (dk == 64 || dk == 128) && (dv == 64 || dv == 128) && ld % 4 == 0 && (((uintptr_t)proj | (uintptr_t)U) & 15) == 0 &&
@@ -643,10 +634,7 @@ extern "C" int fg_retention_chunked(const float *proj, int ld, void *out, int ou
         const size_t sf = ((size_t)2 * RC * (dk + 4) + (size_t)RC * dv + RC * RC) * sizeof(float);
 #define RET_OUT_FAST(DK, DV, TO) do { \
         static FgPerDevice setup; \
-        if (fg_needs_setup(setup)) { \
-            cudaError_t e = cudaFuncSetAttribute(retention_chunk_out_fast<DK, DV, TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024); \
-            if (e != cudaSuccess) return (int)e; \
-        } \
+        if (const int e = fg_allow_shared(setup, retention_chunk_out_fast<DK, DV, TO>, 100 * 1024)) return e; \
         return fg_launch(retention_chunk_out_fast<DK, DV, TO>, dim3(n_chunks, H), dim3(RET_THREADS), sf, stream, proj, ld, (TO *)out, ldo, positions, \
                          (const int *)chunk_row, (const int *)chunk_len, cos_t, sin_t, decay, (const float *)U, H, k_scale, eps, opts); } while (0)
 #define RET_OUT_FAST_T(TO) do { \

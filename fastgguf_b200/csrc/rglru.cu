@@ -473,10 +473,7 @@ static int rglru_step_launch(const float *proj, int ldp, const float *proj_bias,
                              const float *gate_bias, const float *lam, float gain, const int *positions, const int *row_seq, const int *slots,
                              float *state, long long state_stride, void *out, int ldo, int M, int C, int part, cudaStream_t stream) {
     static FgPerDevice setup;
-    if (fg_needs_setup(setup)) {
-        cudaError_t e = cudaFuncSetAttribute(rglru_step_kernel<TW, TO>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-        if (e != cudaSuccess) return (int)e;
-    }
+    if (const int e = fg_allow_shared(setup, rglru_step_kernel<TW, TO>, 200 * 1024)) return e;
     const int stride = (part + 3) / 4 * 4, vec = part % (16 / (int)sizeof(TW)) == 0 && (((uintptr_t)W) & 15) == 0;
     const int vec4 = part % 4 == 0 && ldp % 4 == 0 && state_stride % 4 == 0 &&
                      ((((uintptr_t)proj) | ((uintptr_t)proj_bias) | ((uintptr_t)conv_w) | ((uintptr_t)conv_b) | ((uintptr_t)state)) & 15) == 0;

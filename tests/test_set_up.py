@@ -63,14 +63,11 @@ FIRST_CALLS = """
     import sys, threading
     import torch
     from fastgguf_b200 import ops
+    from fastgguf_b200.ops import fast_gemm
     g = torch.Generator(device="cuda").manual_seed(1)
-    w = ops.mxfp4_quantize(torch.randn(1000, 2048, generator=g, device="cuda"))
-    stack = ops.mxfp4_quantize(torch.randn(2, 1000, 2048, generator=g, device="cuda"))
-    xs = [torch.randn(m, 2048, generator=g, device="cuda").bfloat16() for m in (1, 12, 70, 300)]
-    packed = [ops.mxfp4_quantize(x) for x in xs]
-    cuts = [torch.tensor([0, x.shape[0] // 2, x.shape[0]], dtype=torch.int32, device="cuda") for x in xs]
-    torch.cuda.synchronize()
-    kinds = [lambda i: ops.gemm_mxfp4(xs[i], w), lambda i: ops.gemm_mxfp4_both(packed[i], w), lambda i: ops.gemm_mxfp4_grouped(xs[i], stack, cuts[i])]
+    def random(*shape):
+        return torch.randn(*shape, generator=g, device="cuda") * shape[-1] ** -0.5
+    CALLS
     calls = [(k, i) for i in range(4) for k in kinds] * 2
     together, got, wrong = threading.Barrier(len(calls)), [None] * len(calls), []
 
@@ -84,6 +81,7 @@ FIRST_CALLS = """
                 wrong.append(repr(e))
             torch.cuda.current_stream().synchronize()
 
+    torch.cuda.synchronize()
     threads = [threading.Thread(target=run, args=(j,)) for j in range(len(calls))]
     for t in threads: t.start()
     for t in threads: t.join()
@@ -92,10 +90,27 @@ FIRST_CALLS = """
         wrong = [f"call {j} differs" for j, (k, i) in enumerate(calls) if not torch.equal(got[j], k(i))]
     sys.exit("; ".join(wrong) if wrong else 0)
 """
+KINDS = {
+    "mxfp4": """
+    w, stack = ops.mxfp4_quantize(random(1000, 2048)), ops.mxfp4_quantize(random(2, 1000, 2048))
+    xs = [random(m, 2048).bfloat16() for m in (1, 12, 70, 300)]
+    packed = [ops.mxfp4_quantize(x) for x in xs]
+    cuts = [torch.tensor([0, x.shape[0] // 2, x.shape[0]], dtype=torch.int32, device="cuda") for x in xs]
+    kinds = [lambda i: ops.gemm_mxfp4(xs[i], w), lambda i: ops.gemm_mxfp4_both(packed[i], w), lambda i: ops.gemm_mxfp4_grouped(xs[i], stack, cuts[i])]
+""",
+    "gemm": """
+    w, wide = random(1024, 2048).bfloat16(), random(1024, 2048)
+    xs, x32 = [random(m, 2048).bfloat16() for m in (1, 40, 300, 1500)], [random(m, 2048) for m in (1, 16, 40, 300)]
+    kinds = [lambda i: fast_gemm.gemm_tc(xs[i], w), lambda i: fast_gemm.gemm_tc(xs[i], w, out_dtype=torch.float32),
+             lambda i: fast_gemm.gemm_f32_stream(x32[i], wide) if i < 2 else fast_gemm.gemm_f32(x32[i], wide)]
+""",
+}
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("which", list(KINDS))
 @pytest.mark.parametrize("attempt", range(3))
-def test_first_calls_of_many_threads_at_once(attempt):
-    p = subprocess.run([sys.executable, "-c", textwrap.dedent(FIRST_CALLS)], cwd=ROOT, capture_output=True, text=True, timeout=300)
+def test_first_calls_of_many_threads_at_once(which, attempt):
+    program = textwrap.dedent(FIRST_CALLS.replace("    CALLS\n", KINDS[which].lstrip("\n")))
+    p = subprocess.run([sys.executable, "-c", program], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert p.returncode == 0, p.stderr[-2000:]
