@@ -392,7 +392,8 @@ int fg_attention_prefill_tc_test_hook(long long wait_limit_cycles, int skip_copy
 /* fg_attention_decode_noalloc: see fastgguf_noalloc.h */
 
 /* ---- libfg_mx: matrices in microscaled 4-bit floating point.  data [rows, K / 2] bytes, scales [ceil(rows / 128), ceil(K / 128), 32, 4, 4]
-   bytes (mxfp4.cuh), both 16-byte aligned; K a multiple of 32; strides count numbers */
+   bytes (mxfp4.cuh), both 16-byte aligned; exponents of rows and blocks past the matrix may be any byte but 255; K a multiple of 32; strides count
+   numbers */
 /* mats matrices [R, K] of dtype (rows ldx, matrices x_stride apart) to data and scales, one matrix after another */
 int fg_mxfp4_quantize(const void *x, int dtype, long long ldx, long long x_stride, void *data, void *scales, int mats, int R, int K,
                       cudaStream_t stream);
@@ -402,14 +403,15 @@ int fg_mxfp4_rows(const void *data, const void *scales, const int *rows, void *o
 /* out (+)= x w^T: x [M, K] bfloat16, w [N, K]; out bfloat16 or float32, accumulate: float32 alone */
 int fg_gemm_mxfp4(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
                   int M, int N, int K, cudaStream_t stream);
-/* the same with the kernel named: form 0 by the rule, 1 for few rows, 2 tiles, 3 tiles of pairs of CTAs; bn tokens a tile (a multiple of 16,
-   up to 256), K over `splits` CTAs (form 2, up to 8) */
+/* the same with the kernel named: form 0 by the rule (bn and splits are not read), 1 for few rows (the same), 2 tiles, 3 tiles of pairs of CTAs; bn
+   tokens a tile up to 256, a multiple of 16 (form 2) or 32 (form 3); K over `splits` CTAs, 1 to 8 (form 2) or 1 (form 3) */
 int fg_gemm_mxfp4_ext(const void *x, long long ldx, const void *w, const void *scales, void *out, int out_dtype, long long ldo, int accumulate,
                       int M, int N, int K, int form, int bn, int splits, cudaStream_t stream);
 /* rows offsets[e] <= m < offsets[e + 1] (device) with matrix e of a stack; rows of no run are not written */
 int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w, const void *scales, const int *offsets, int experts, void *out,
                           int out_dtype, long long ldo, int accumulate, int M, int N, int K, cudaStream_t stream);
-/* the same with x in the format too; ext: bn tokens a tile and `splits` CTAs that share K (0: by the rule) */
+/* out (+)= x w^T with x in the format too.  ext: bn 0 chooses both by the rule; else bn tokens a tile - 128, 256, or a multiple of 16 up to 256 that takes all
+   rows - and `splits` CTAs, 1 to 8, that share K */
 int fg_gemm_mxfp4_both(const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int out_dtype, long long ldo,
                        int accumulate, int M, int N, int K, cudaStream_t stream);
 int fg_gemm_mxfp4_both_ext(const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int out_dtype, long long ldo,

@@ -239,8 +239,8 @@ static int both_plan(int M, int N, int K, int &bn, int &S) {
     return 0;
 }
 
-// x, w and their exponents in the format; bn, splits: 0 by the rule, else (tests, measurements) tokens a tile - a multiple of 128 up to 256, or a multiple of 16
-// not below M rounded up to one - and CTAs that share K
+// x, w and their exponents in the format; bn 0: both by the rule, else (tests, measurements) tokens a tile - 128, 256, or a multiple of 16 up to 256 that takes
+// all rows - and CTAs that share K, 1 to 8
 extern "C" int fg_gemm_mxfp4_both_ext(const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int out_dtype, long long ldo,
                                       int accumulate, int M, int N, int K, int bn, int splits, cudaStream_t stream) {
     MxBoth a = {};

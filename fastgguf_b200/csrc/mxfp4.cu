@@ -159,7 +159,7 @@ mxfp4_rows_kernel(const uint8_t *data, const uint8_t *scales, const int *rows, T
         w[p] = 0;
         e[p] = 255;
         if (at < total) {
-            const unsigned i = per_row == 1 ? at : (unsigned)__umul64hi(at, over);
+            const unsigned i = (unsigned)__umul64hi(at, over);
             const int c = (int)(at - i * per_row) * 8, r = rows ? rows[r0 + i] : r0 + (int)i;
             to[p] = (long long)(r0 + (int)i) * ldo + c;
             if (r >= 0 && r < R) {

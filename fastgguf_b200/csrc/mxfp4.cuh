@@ -5,7 +5,8 @@
 // low half of byte i; `scales` [ceil(rows / 128), ceil(K / 128), 32, 4, 4] bytes: block b of row r at
 // [r / 128, b / 4, r % 32, r / 32 % 4, b % 4] - tiles of 512 bytes in the order in which a block-scaled tensor instruction
 // wants the exponents of 128 rows x 128 numbers, and in which a warp that takes eight rows of each quarter of a tile finds
-// its exponents in 128 neighbouring bytes.  K is a multiple of 32; exponents of rows and blocks past the matrix are padding.
+// its exponents in 128 neighbouring bytes.  K is a multiple of 32; exponents of rows and blocks past the matrix are padding, any
+// byte but 255.
 #pragma once
 #include "common.cuh"
 

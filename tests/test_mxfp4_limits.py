@@ -245,3 +245,13 @@ def test_quantising_more_tiles_than_a_grids_second_dimension(dtype, lead, rows, 
         back = ops.mxfp4_rows(q)
         for at in (0, 127, 4194304, rows - 300):
             assert torch.equal(back[at:at + 300].double().cpu(), plain.rounded(x[at:at + 300])[0])
+
+
+def test_named_kernels_refuse_what_the_header_does_not_allow():
+    """Before they touch the device or the memory (the addresses here are none)."""
+    from ctypes import c_void_p
+    L, refused, at = ops.lib("mx"), 10002, c_void_p(1 << 20)                      # (FG_ERR_BAD_SIZE)
+    for form, bn, splits in [(2, 0, 1), (2, 24, 1), (2, 272, 1), (2, 64, 0), (2, 64, 9), (3, 48, 1), (3, 64, 2), (3, 64, 0), (4, 64, 1), (-1, 64, 1)]:
+        assert L.fg_gemm_mxfp4_ext(at, 64, at, at, at, 1, 64, 0, 100, 64, 64, form, bn, splits, None) == refused, (form, bn, splits)
+    for bn, splits in [(128, 0), (128, 9), (112, 0), (96, 1), (24, 1), (272, 1)]:  # (96: does not take 100 rows)
+        assert L.fg_gemm_mxfp4_both_ext(at, at, at, at, at, 1, 64, 0, 100, 64, 64, bn, splits, None) == refused, (bn, splits)
