@@ -39,10 +39,13 @@ __device__ __forceinline__ void mx_store(const MxGemm &a, int m, int n, float v)
 // in shared memory in the lanes' order.  Every lane copies what it will use itself, asynchronously and three chunks ahead (104 KB in flight
 // on an SM, with no registers held for them), so the ring needs no barrier.
 //
-// What bounds it: instructions.  At the memory's rate an SM gets a chunk's 2,176 bytes of 32 rows every 92 cycles, in which its four
-// schedulers issue 368; unpacking them takes 192, the MMAs, loads and addresses some 70.  Measured: 8 x 28,672 x 4,096 22.5 us (2.8 TB/s), one row of
-// 128,256 x 2,048 35.1 (4.0).  Sixteen warps do not hide all of their waits: with two groups of eight (23.5 us) the schedulers issued in 54 % of active
-// cycles, DRAM was at 29 %.
+// What bounds it: neither memory nor issue alone.  At the memory's rate an SM gets a chunk's 2,176 bytes of 32 rows every 92 cycles, in which its four
+// schedulers issue 368; unpacking them takes 192, the MMAs, loads and addresses some 70.  Measured: 8 x 28,672 x 4,096 22.6 us (2.8 TB/s): 896 units on 592
+// groups of warps are two rounds for 1.51, the schedulers issue in 55 % of active cycles, DRAM is at 30 %, and a warp that does not issue waits for its copies, for
+// a busy pipe and for its last result in about equal parts (1.1, 1.1 and 1.0 cycles an instruction).  One row of 128,256 x 2,048 35.1 us (4.0 TB/s):
+// 6.8 rounds of seven, issue in 65 %, DRAM at 45 %.
+// Blocks with exponents above 125 (a largest number of 2 and more: a table of unit variance has them in 78 % of its blocks) take mx_times_rest, a warp's chunk
+// as a whole: 8 x 28,672 x 4,096 41.4 us, one row of 128,256 x 2,048 68.5, 8 x 8,192 x 2,048 8.3 from 6.0.
 //
 // A CTA is two groups of eight warps or four of four; a group takes a unit of 32 rows at a time, its warps a chunk each in turn.  x is staged once for all the
 // units of a CTA (in parts, for each unit again, where K is longer than the room).  The warps' sums are added in shared memory, those of a cluster's
@@ -321,8 +324,9 @@ static int launch_stream(const MxGemm &a, int y, int busy /* of the y, that have
 // Unpacking is bound by the integer pipe when enough warps hide the waits around it: with two warps a scheduler, half a stage each, a
 // stage's took 1,500 cycles beside the 1,024 of its MMAs at 256 tokens (2,048 x 8,192 x 4,096: 133 us; with four: 94).  At few tokens a stage
 // takes some 650 cycles: unpacking and the chain from a free slot to the next full one, beside MMAs of 46 cycles each.
-// Measured: 77 x 8,191 x 2,080 9.5 us; 256 x 8,192 x 4,096 17.3 us (995 TFLOP/s); 2,048 x 14,336 x 4,096 162 us (1,482 TFLOP/s) in a short run, 181 at the
-// power limit; at 2,048 x 28,672 x 4,096 the tensor pipe is busy in 86 % of active cycles.
+// Measured: 77 x 8,191 x 2,080 10.1 us; 256 x 8,192 x 4,096 18.1 us (950 TFLOP/s); 2,048 x 14,336 x 4,096 162 us (1,482 TFLOP/s) in a short run, 184 to 190 at
+// the power limit; at 2,048 x 28,672 x 4,096 the tensor pipe is busy in 86 % of active cycles.  Where every block has an exponent above 125: 11.1, 22.4 and
+// 167 to 190 us.
 //
 // One CTA an SM walks the tiles.  PAIR: two CTAs of a cluster take 256 weight rows x BN tokens (tcgen05.mma.cta_group::2); each unpacks its
 // own 128 rows and brings half of the tokens, which halves the bytes an SM receives per MMA.  With few tiles a cluster of single CTAs splits
@@ -776,8 +780,8 @@ extern "C" int fg_gemm_mxfp4_grouped(const void *x, long long ldx, const void *w
     a.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     if (experts <= TILE_MAX_EXPERTS && tile_ok(a)) {
         // The runs' lengths are known on the device alone: a tile's width by their mean, with room for a router that prefers some experts (32 experts
-        // of 2,048 x 2,048, us at 16 | 32 | 64 | 128 tokens a tile: mean 2: 15.3 | 16.3 | 16.5 | -; mean 4: 27.6 | 22.4 | 23.1 | 25.1;
-        // mean 16: 41.0 | 29.0 | 29.7 | 32.3; mean 32: 60.7 | 41.5 | 36.1 | 33.1; eight experts, mean 37: 21.5 | 16.0 | 10.5 | 11.5)
+        // of 2,048 x 2,048, us at 16 | 32 | 64 | 128 tokens a tile: mean 2: 15.6 | 16.4 | 17.0 | 18.4; mean 4: 27.9 | 22.6 | 23.3 | 25.2;
+        // mean 16: 40.7 | 29.0 | 29.7 | 32.7; mean 32: 60.3 | 41.4 | 35.9 | 33.0; eight experts, mean 37: 22.1 | 16.5 | 10.8 | 11.9)
         const long long mean = ((long long)M + experts - 1) / experts;
         if (mean <= 2) return launch_tiles<false>(a, 16, 1, stream);
         return launch_tiles<true>(a, mean <= 8 ? 32 : mean <= 20 ? 64 : 128, 1, stream);

@@ -12,8 +12,8 @@
 //   warps 2-9   epilogue, two to a lane group: the accumulator goes to registers at once and is free for the next tile while they store
 //
 // One CTA an SM walks the tiles; with few tiles a cluster of CTAs splits K and sums through distributed shared memory, in rank order.
-// What bounds it: the feed of the tensor pipe, busy in 65 % of active cycles at 2,048 x 28,672 x 4,096.  Measured: 200 x 8,192 x 2,048 8.1 us;
-// 2,048 x 14,336 x 4,096 58.0 to 62.0 us (3.9 to 4.1 PFLOP/s).
+// What bounds it: the feed of the tensor pipe, busy in 65 % of active cycles at 2,048 x 28,672 x 4,096.  Measured: 200 x 8,192 x 2,048 6.8 to 8.7 us;
+// 1 to 16 x 8,192 x 4,096 8.0; 2,048 x 14,336 x 4,096 54 to 63 us (4.4 to 3.8 PFLOP/s).
 #pragma once
 
 #define BOTH_ROWS 128

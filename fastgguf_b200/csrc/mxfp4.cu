@@ -8,7 +8,7 @@
 //
 // A CTA takes 128 rows x 128 numbers.  A thread reads 32 bytes of a row at a time, 8 float32 or 16 bfloat16 numbers; the four or two threads of
 // a block find its maximum by shuffles.  The exponents of the tile are 512 neighbouring bytes, gathered in shared memory.
-// 14,336 x 4,096: 47.0 us from float32 (5.7 TB/s), 30.8 from bfloat16 (4.8).
+// 14,336 x 4,096: 47.1 us from float32 (5.6 TB/s), 31.0 from bfloat16 (4.8).
 __device__ __forceinline__ void load_piece(const float *p, bool vec, float (&v)[8]) {
     if (vec)
         asm("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -119,8 +119,8 @@ extern "C" int fg_mxfp4_quantize(const void *x, int dtype, long long ldx, long l
 // ---------------------------------------------------------------------------- rows
 // out[i] = scale * row rows[i] (null: row i).  A piece is eight numbers, which lie in one block: four bytes in, 16 or 32 out.  A thread takes four
 // pieces, 256 apart, and asks for all of them before it converts the first.  The number itself is exact in either type; a scale other than 1 rounds
-// once.  A row index outside the matrix gives a row of NaN.  14,336 x 4,096: 42.9 us to float32 (6.2 TB/s), 37.7 to bfloat16 (3.9); 4,001 picked rows
-// of 2,048 6.9 us (5.4).
+// once.  A row index outside the matrix gives a row of NaN.  14,336 x 4,096: 42.9 us to float32 (6.2 TB/s), 36.0 to bfloat16 (4.1: the schedulers
+// issue in 82 % of cycles); 4,001 picked rows of 2,048 6.9 us to float32 (5.4), 6.3 to bfloat16.
 #define ROWS_PIECES 4
 __device__ __forceinline__ void store8(float *p, bool vec, const float (&v)[8]) {
     if (vec)

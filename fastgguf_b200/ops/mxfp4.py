@@ -82,7 +82,14 @@ class Mxfp4:
 
     @classmethod
     def from_exponents(cls, data: torch.Tensor, exponents: torch.Tensor) -> "Mxfp4":
-        """From exponents row by row, uint8 [.., rows, K / 32]."""
+        """From exponents row by row, uint8 [.., rows, K / 32].
+
+        Model files may order a block's sixteen bytes otherwise: where byte j holds number j in its low half and number j + 16 in its high half (GGUF's
+        MXFP4 blocks, whose exponent is this one), ``raw`` [.., rows, K / 32, 16] of such bytes becomes ``data`` by
+
+            codes = torch.cat([raw & 15, raw >> 4], -1)
+            data = (codes[..., 0::2] | codes[..., 1::2] << 4).flatten(-2)
+        """
         rows, k = data.shape[-2], 2 * data.shape[-1]
         if exponents.dtype != torch.uint8 or k % BLOCK or exponents.shape != (*data.shape[:-1], k // BLOCK):
             raise KernelError(f"Mxfp4: exponents are uint8 [.., rows, K / {BLOCK}], got {exponents.dtype} {tuple(exponents.shape)} for data {tuple(data.shape)}")

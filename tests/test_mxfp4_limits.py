@@ -255,3 +255,15 @@ def test_named_kernels_refuse_what_the_header_does_not_allow():
         assert L.fg_gemm_mxfp4_ext(at, 64, at, at, at, 1, 64, 0, 100, 64, 64, form, bn, splits, None) == refused, (form, bn, splits)
     for bn, splits in [(128, 0), (128, 9), (112, 0), (96, 1), (24, 1), (272, 1)]:  # (96: does not take 100 rows)
         assert L.fg_gemm_mxfp4_both_ext(at, at, at, at, at, 1, 64, 0, 100, 64, 64, bn, splits, None) == refused, (bn, splits)
+
+
+def test_blocks_that_keep_their_halves_apart_are_reordered_as_the_text_says():
+    """Byte j of a block: number j below, number j + 16 above."""
+    numbers = torch.randint(0, 16, (3, 5, 32), generator=_gen(1), dtype=torch.uint8)         # codes [rows, blocks, 32]
+    raw = numbers[..., :16] | numbers[..., 16:] << 4
+    codes = torch.cat([raw & 15, raw >> 4], -1)
+    data = (codes[..., 0::2] | codes[..., 1::2] << 4).flatten(-2)
+    e = torch.randint(100, 140, (3, 5), generator=_gen(2), dtype=torch.uint8)
+    w = Mxfp4.from_exponents(data, e)
+    want = plain.VALUES[numbers.long()] * torch.pow(torch.tensor(2.0, dtype=torch.float64), e.double() - 127)[..., None]
+    assert torch.equal(plain.of(w), want.reshape(3, 160))
